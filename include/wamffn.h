@@ -41,6 +41,8 @@
  *                                  WAMInfer/_triton_attention.py:327-334
  *   wamffn_current_frame_attention <- op wam_infer::current_frame_attention_v1
  *                                  WAMInfer/_triton_attention.py:429-484
+ *   wamffn_qk_norm_rope         <- the Q/K RMSNorm + RoPE kernel
+ *                                  WAMInfer/_triton_inference.py:13-112
  */
 #ifndef WAMFFN_H
 #define WAMFFN_H
@@ -528,6 +530,139 @@ typedef struct wamffn_current_frame_args {
 } wamffn_current_frame_args;
 
 int wamffn_current_frame_attention(void* stream, const wamffn_current_frame_args* args);
+
+/* ------------------------------------------------------------------------
+ * Norm of queries and keys with the position rotation in the same pass (the
+ * step between the QKV projection and the attention; the reference's whole-row
+ * form is WAMInfer/_triton_inference.py:13-112):
+ *   r = rsqrt(mean(x^2) + eps) over one head, or over the whole row
+ *   y = x r weight;  pair (a, b) of a head -> (y_a c - y_b s, y_a s + y_b c)
+ * c + i s = rope[position, i], i < pairs; (a, b) = (2i, 2i+1) when interleaved,
+ * else (i, i + pairs); dims past 2 pairs are not turned.  fp32 throughout,
+ * rounded to bf16 once.
+ * q: [batch, rows, heads * head_dim], k: [batch, rows, kv_heads * head_dim]
+ * (data NULL with kv_heads 0: queries only), row and batch strides in elements,
+ * multiples of 8.  Weights: head_dim values, or with whole_row the row's width.
+ * rope: complex64 [table_rows, >= pairs], table_stride complex elements between
+ * rows (even), 16-byte aligned; pairs a multiple of 4, <= head_dim / 2; NULL: no
+ * rotation.  positions: int32 / int64 (position_bytes 4 / 8), position_stride
+ * elements between batches (0: shared); NULL: the row's index.  A position
+ * outside the table reads nothing and gives a row of NaN.
+ * Outputs contiguous.  head_dim 64, 128 or 256; with whole_row
+ * (heads + kv_heads) * head_dim <= 32768.
+ * ---------------------------------------------------------------------- */
+typedef struct wamffn_qk_rope_args {
+  wamffn_rows_view q, k;
+  const void* q_weight;
+  const void* k_weight;
+  const void* rope;
+  int64_t table_stride;
+  const void* positions;
+  int64_t position_stride;
+  void* q_out;
+  void* k_out;
+  int position_bytes;
+  int table_rows;
+  int pairs;
+  int batch;
+  int rows;
+  int heads;
+  int kv_heads;
+  int head_dim;
+  int whole_row;
+  int interleaved;
+  float eps;
+} wamffn_qk_rope_args;
+
+int wamffn_qk_norm_rope(void* stream, const wamffn_qk_rope_args* args);
+
+/* ------------------------------------------------------------------------
+ * Key / value cache in 8 bits.  No counterpart in the reference (its cached
+ * prefix is bf16, WAMInfer/_triton_attention.py:337-484).  Blocks of
+ * WAMFFN_CACHE_BLOCK tokens, head dim 128:
+ *   keys, values   [blocks, kv_heads, 64, 128] e4m3, 16-byte aligned
+ *   *_scales       [blocks, kv_heads] fp32, powers of two; a row is value * scale
+ *   block_table    [batch, width] int32 (table_stride elements between
+ *                  sequences): the block of rows [64 i, 64 i + 64)
+ *   lengths        [batch] int32, rows held
+ *   tickets        [batch] int32 work words, zero when no append is running
+ *   status         device word for WAMFFN_DEV_* bits, or NULL
+ * A block may stand in several tables for reading; one that is appended to must
+ * stand in one.  Two appends to one cache must not overlap in time.
+ * ---------------------------------------------------------------------- */
+#define WAMFFN_CACHE_BLOCK 64
+
+typedef struct wamffn_cache_view {
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int32_t* lengths;
+  int32_t* tickets;
+  uint32_t* status;
+  int blocks;
+  int kv_heads;
+  int batch;
+  int width;
+} wamffn_cache_view;
+
+/* Stores rows k, v [batch, rows, kv_heads * 128] bf16 (strides in elements,
+ * multiples of 8) at row at[b] of sequence b (at NULL: lengths[b]) and sets
+ * lengths[b] = at[b] + counts[b]; counts NULL: rows; rows past counts[b] (a
+ * padded batch) are not stored.  at[b] < lengths[b] replaces the rows from there
+ * on.  Scale of a block and head: 2^e, the least e >= -60 with
+ * |x| <= 448 * 2^e for its finite values; a block that holds rows in front of
+ * the new ones keeps at least the scale it has, and when that grows those rows
+ * are turned over to it.  Values are rounded to the nearest e4m3 (even on
+ * ties); infinities become +-448 * 2^e, NaN stays.  A sequence whose rows do not
+ * fit (at[b] outside [0, lengths[b]], past width * 64 rows, a block id outside
+ * [0, blocks)) is left unchanged and sets WAMFFN_DEV_BAD_INDEX. */
+typedef struct wamffn_cache_append_args {
+  wamffn_cache_view cache;
+  wamffn_rows_view k, v;
+  const int32_t* counts;
+  const int32_t* at;
+  int rows;
+} wamffn_cache_append_args;
+
+int wamffn_cache_append(void* stream, const wamffn_cache_append_args* args);
+
+/* Rows [start, start + count) of every sequence as bf16 (exactly the held
+ * values), k and v [batch, count, kv_heads * 128] contiguous; zeros outside
+ * [0, lengths[b]).  start: int32 [batch], or NULL for start_all. */
+typedef struct wamffn_cache_read_args {
+  wamffn_cache_view cache;
+  const int32_t* start;
+  void* k;
+  void* v;
+  int start_all;
+  int count;
+} wamffn_cache_read_args;
+
+int wamffn_cache_read(void* stream, const wamffn_cache_read_args* args);
+
+/* out[b, i, h] = softmax over the rows j that query i sees of
+ * (q[b, i, h] . k[j] / sqrt(128)) . v[j]: j < lengths[b], or with causal
+ * j < lengths[b] - nq + i + 1 (the queries are the cache's last nq rows); a row
+ * that sees nothing is zeros.  q: [batch, nq, heads * 128] bf16 (strides
+ * multiples of 8), heads a multiple of the cache's kv_heads: query heads
+ * [g * heads / kv_heads, ...) share key head g.  out contiguous.  fp32 scores,
+ * maximum, sums; the probabilities of the value product in f16.  A block id
+ * outside the pool is left out and sets WAMFFN_DEV_BAD_INDEX.  key_split: CTAs
+ * that share a row tile's keys, 0 picks it (1, 2, 4 or 8 forces it). */
+typedef struct wamffn_cache_attention_args {
+  wamffn_cache_view cache;
+  wamffn_rows_view q;
+  void* out;
+  int nq;
+  int heads;
+  int causal;
+  int key_split;
+} wamffn_cache_attention_args;
+
+int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* args);
 
 #ifdef __cplusplus
 }

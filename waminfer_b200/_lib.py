@@ -13,6 +13,8 @@ import os
 import threading
 from pathlib import Path
 
+import torch
+
 LIB_PATH = Path(__file__).with_name("libwamffn.so")
 
 WAMFFN_OK = 0
@@ -55,6 +57,10 @@ EXPORTED_SYMBOLS = (
     "wamffn_masked_attention",
     "wamffn_joint_first_frame_attention",
     "wamffn_current_frame_attention",
+    "wamffn_qk_norm_rope",
+    "wamffn_cache_append",
+    "wamffn_cache_read",
+    "wamffn_cache_attention",
     "wamffn_rgb_mandatory",
     "wamffn_select_tokens",
     "wamffn_pack_weight",
@@ -160,6 +166,58 @@ class CurrentFrameArgs(ctypes.Structure):
         ("head_dim", ctypes.c_int),
         ("key_split", ctypes.c_int),
     ]
+
+
+class QkRopeArgs(ctypes.Structure):
+    """Mirror of ``wamffn_qk_rope_args``."""
+
+    _fields_ = [
+        ("q", RowsView),
+        ("k", RowsView),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("rope", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        *[(name, ctypes.c_int) for name in ("position_bytes", "table_rows", "pairs", "batch", "rows", "heads",
+                                            "kv_heads", "head_dim", "whole_row", "interleaved")],
+        ("eps", ctypes.c_float),
+    ]
+
+
+class CacheView(ctypes.Structure):
+    """Mirror of ``wamffn_cache_view``."""
+
+    _fields_ = [
+        *[(name, ctypes.c_void_p) for name in ("keys", "values", "key_scales", "value_scales", "block_table")],
+        ("table_stride", ctypes.c_int64),
+        *[(name, ctypes.c_void_p) for name in ("lengths", "tickets", "status")],
+        *[(name, ctypes.c_int) for name in ("blocks", "kv_heads", "batch", "width")],
+    ]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    """Mirror of ``wamffn_cache_append_args``."""
+
+    _fields_ = [("cache", CacheView), ("k", RowsView), ("v", RowsView), ("counts", ctypes.c_void_p),
+                ("at", ctypes.c_void_p), ("rows", ctypes.c_int)]
+
+
+class CacheReadArgs(ctypes.Structure):
+    """Mirror of ``wamffn_cache_read_args``."""
+
+    _fields_ = [("cache", CacheView), ("start", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("start_all", ctypes.c_int), ("count", ctypes.c_int)]
+
+
+class CacheAttentionArgs(ctypes.Structure):
+    """Mirror of ``wamffn_cache_attention_args``."""
+
+    _fields_ = [("cache", CacheView), ("q", RowsView), ("out", ctypes.c_void_p), ("nq", ctypes.c_int),
+                ("heads", ctypes.c_int), ("causal", ctypes.c_int), ("key_split", ctypes.c_int)]
 
 
 class BlockArgs(ctypes.Structure):
@@ -280,6 +338,10 @@ def _declare(lib):
     lib.wamffn_masked_attention.argtypes = [vp, ctypes.POINTER(AttentionArgs)]
     lib.wamffn_joint_first_frame_attention.argtypes = [vp, ctypes.POINTER(JointAttentionArgs)]
     lib.wamffn_current_frame_attention.argtypes = [vp, ctypes.POINTER(CurrentFrameArgs)]
+    lib.wamffn_qk_norm_rope.argtypes = [vp, ctypes.POINTER(QkRopeArgs)]
+    lib.wamffn_cache_append.argtypes = [vp, ctypes.POINTER(CacheAppendArgs)]
+    lib.wamffn_cache_read.argtypes = [vp, ctypes.POINTER(CacheReadArgs)]
+    lib.wamffn_cache_attention.argtypes = [vp, ctypes.POINTER(CacheAttentionArgs)]
     lib.wamffn_rgb_mandatory.argtypes = [vp, vp, vp, i, i, i, i, vp]
     lib.wamffn_select_tokens.argtypes = [vp, ctypes.POINTER(SelectArgs)]
     lib.wamffn_pack_weight.argtypes = [vp, vp, vp, i, i]
@@ -316,6 +378,15 @@ def check(status: int) -> None:
     if status != WAMFFN_OK:
         message = lib().wamffn_last_error().decode(errors="replace")
         raise WamffnError(status, message)
+
+
+def launch(entry, device: int, args) -> None:
+    """Calls entry(current stream of `device`, args) with `device` current."""
+    if torch._C._cuda_getDevice() == device:
+        check(entry(torch._C._cuda_getCurrentRawStream(device), args))
+    else:
+        with torch.cuda.device(device):
+            check(entry(torch._C._cuda_getCurrentRawStream(device), args))
 
 
 def launch_count() -> int:

@@ -1,0 +1,195 @@
+"""Key / value cache in 8 bits and the attention over it, on libwamffn.
+
+The bf16 attention ops (``waminfer_b200/attention.py``) read their cached prefix
+and text context in 16 bits.  ``KVCache8`` keeps such rows in e4m3 with one
+power-of-two scale for each block of 64 tokens and head: half the memory and half the
+bytes an attention over them has to read.
+
+    cache = KVCache8(batch=4, capacity=4096, kv_heads=24, device="cuda")
+    cache.append(k, v)                       # [4, rows, 24 * 128] bf16, after the norm and rotation
+    out = cache.attend(q, heads=24)          # [4, nq, 24 * 128]
+    k, v = cache.read(120)                   # rows back as bf16, e.g. for current_frame_attention
+
+Rows that change at every step (the current frame through the Euler updates)
+are replaced in place: ``append(..., at=start)``.  Everything is on the device
+(lengths, block table), so all calls can be captured into CUDA graphs.
+Inference only: no backward pass.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from waminfer_b200 import _lib
+
+BLOCK = 64
+HEAD_DIM = 128
+FORMAT = torch.float8_e4m3fn
+
+
+def _rows(t: torch.Tensor, name: str, batch: int, width: int, device: torch.device) -> torch.Tensor:
+    """A [batch, rows, width] bf16 operand that the kernels can read in place, else a copy."""
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.device != device:
+        raise ValueError(f"{name} must be a bf16 tensor [batch, rows, heads * {HEAD_DIM}] on {device}")
+    if t.shape[0] != batch or t.shape[2] != width:
+        raise ValueError(f"{name} {tuple(t.shape)}: expected [{batch}, rows, {width}]")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("the 8-bit cache has no backward pass: run it with gradients disabled")
+    sb, sr, se = t.stride()
+    if se != 1 or sb % 8 or sr % 8 or t.data_ptr() % 16 or (sr < width and t.shape[1] > 1):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _view(t: torch.Tensor) -> _lib.RowsView:
+    return _lib.RowsView(t.data_ptr(), t.stride(1), t.stride(0))
+
+
+def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}, not "
+                         f"{t.dtype} {list(t.shape)} on {t.device}")
+
+
+class KVCache8:
+    """Keys and values of ``batch`` sequences in e4m3 blocks of 64 tokens, head dim 128.
+
+    ``capacity`` rows a sequence; ``blocks`` sizes the pool (default: every
+    sequence's full capacity, with a table that gives each its own blocks).  With a
+    pool of its own size the caller fills ``block_table`` (int32 [batch, width])
+    before rows reach those places; a block may stand in several tables for reading
+    (a shared prefix), one that rows are appended to in one only.
+
+    Tensors: ``keys``, ``values`` [blocks, kv_heads, 64, 128] float8_e4m3fn;
+    ``key_scales``, ``value_scales`` float32 [blocks, kv_heads], powers of two (a
+    row is value * scale); ``block_table``; ``lengths`` int32 [batch], rows held
+    (lowering an entry drops rows).  Calls on one cache follow the stream order of
+    one stream at a time.
+    """
+
+    def __init__(self, batch: int, capacity: int, kv_heads: int, device, blocks: int | None = None):
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("the 8-bit cache lives on a CUDA device")
+        if batch < 1 or capacity < 1 or kv_heads < 1 or (blocks is not None and blocks < 1):
+            raise ValueError(f"batch={batch} capacity={capacity} kv_heads={kv_heads} blocks={blocks}")
+        width = -(-capacity // BLOCK)
+        pool = batch * width if blocks is None else blocks
+        shape = (pool, kv_heads, BLOCK, HEAD_DIM)
+        if blocks is None:
+            table = torch.arange(pool, dtype=torch.int32, device=device).view(batch, width)
+        else:
+            table = torch.full((batch, width), -1, dtype=torch.int32, device=device)
+        self._hold(torch.zeros(shape, dtype=torch.uint8, device=device).view(FORMAT),
+                   torch.zeros(shape, dtype=torch.uint8, device=device).view(FORMAT),
+                   torch.ones(shape[:2], dtype=torch.float32, device=device),
+                   torch.ones(shape[:2], dtype=torch.float32, device=device),
+                   table, torch.zeros(batch, dtype=torch.int32, device=device))
+
+    @classmethod
+    def of(cls, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+           block_table: torch.Tensor, lengths: torch.Tensor) -> "KVCache8":
+        """A cache over tensors that the caller holds (laid out as the class describes)."""
+        self = cls.__new__(cls)
+        self._hold(keys, values, key_scales, value_scales, block_table, lengths)
+        return self
+
+    def _hold(self, keys, values, key_scales, value_scales, block_table, lengths):
+        if keys.dim() != 4 or not keys.is_cuda:
+            raise ValueError(f"keys must be a CUDA tensor [blocks, kv_heads, {BLOCK}, {HEAD_DIM}]")
+        device, (pool, kv_heads) = keys.device, keys.shape[:2]
+        if block_table.dim() != 2:
+            raise ValueError("block_table must be [batch, width]")
+        batch, width = block_table.shape
+        for name, t in (("keys", keys), ("values", values)):
+            _check(name, t, FORMAT, (pool, kv_heads, BLOCK, HEAD_DIM), device)
+        for name, t in (("key_scales", key_scales), ("value_scales", value_scales)):
+            _check(name, t, torch.float32, (pool, kv_heads), device)
+        _check("block_table", block_table, torch.int32, (batch, width), device)
+        _check("lengths", lengths, torch.int32, (batch,), device)
+        if min(pool, kv_heads, batch, width) < 1:
+            raise ValueError("the cache is empty")
+        self.keys, self.values = keys, values
+        self.key_scales, self.value_scales = key_scales, value_scales
+        self.block_table, self.lengths = block_table, lengths
+        self.batch, self.width, self.kv_heads, self.device = batch, width, kv_heads, device
+        self._work = torch.zeros(batch + 1, dtype=torch.int32, device=device)  # tickets, status word
+        self._view = _lib.CacheView(
+            keys=keys.data_ptr(), values=values.data_ptr(), key_scales=key_scales.data_ptr(),
+            value_scales=value_scales.data_ptr(), block_table=block_table.data_ptr(), table_stride=width,
+            lengths=lengths.data_ptr(), tickets=self._work.data_ptr(), status=self._work.data_ptr() + 4 * batch,
+            blocks=pool, kv_heads=kv_heads, batch=batch, width=width)
+
+    @property
+    def capacity(self) -> int:
+        """Rows that a sequence can hold."""
+        return self.width * BLOCK
+
+    def _index(self, name: str, t: torch.Tensor) -> int:
+        _check(name, t, torch.int32, (self.batch,), self.device)
+        return t.data_ptr()
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None = None,
+               at: torch.Tensor | None = None) -> None:
+        """Stores k, v [batch, rows, kv_heads * 128] bf16 behind each sequence's
+        rows (``at``, int32 [batch]: from that row on, replacing what was there)
+        and moves ``lengths``.  ``counts`` (int32 [batch]) says how many of the
+        rows are real in a padded batch.
+
+        A block's scale is the least 2^e with |x| <= 448 * 2^e (e >= -60) over
+        its finite values; infinities are stored as the largest value, NaN stays.
+        When a later row raises the scale of a block, the rows in front of it are
+        rounded to the new one.  A sequence whose rows do not fit (past capacity, ``at``
+        beyond its length, a block id outside the pool) keeps what it had, and
+        ``status`` reports it."""
+        width = self.kv_heads * HEAD_DIM
+        k, v = _rows(k, "k", self.batch, width, self.device), _rows(v, "v", self.batch, width, self.device)
+        if k.shape != v.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        if k.shape[1] == 0:
+            raise ValueError("append needs at least one row (counts may be zero)")
+        args = _lib.CacheAppendArgs(self._view, _view(k), _view(v), None if counts is None else self._index(
+            "counts", counts), None if at is None else self._index("at", at), k.shape[1])
+        _lib.launch(_lib.lib().wamffn_cache_append, self.device.index, ctypes.byref(args))
+
+    def read(self, count: int, start: int | torch.Tensor = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows [start, start + count) of every sequence as bf16, k and v
+        [batch, count, kv_heads * 128]; ``start`` a number or int32 [batch].
+        Rows that a sequence does not hold are zeros."""
+        tensor = isinstance(start, torch.Tensor)
+        if count < 1 or (not tensor and not 0 <= start < 2 ** 31):
+            raise ValueError(f"read of {count} rows from {start}")
+        k = torch.empty((self.batch, count, self.kv_heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
+        args = _lib.CacheReadArgs(self._view, self._index("start", start) if tensor else None, k.data_ptr(),
+                                  v.data_ptr(), 0 if tensor else start, count)
+        _lib.launch(_lib.lib().wamffn_cache_read, self.device.index, ctypes.byref(args))
+        return k, v
+
+    def attend(self, q: torch.Tensor, heads: int, causal: bool = False, key_split: int = 0) -> torch.Tensor:
+        """softmax(q . k / sqrt(128)) . v over each sequence's rows, q [batch,
+        nq, heads * 128] bf16, ``heads`` a multiple of ``kv_heads`` (query heads
+        [g * heads / kv_heads, ...) share key head g).  ``causal``: the queries
+        are the cache's last nq rows, query i sees rows < length - nq + i + 1.  A
+        row that sees nothing is zeros.  key_split: CTAs sharing a query tile's
+        keys (0 = chosen; 1, 2, 4, 8)."""
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"heads={heads} must be a multiple of the cache's {self.kv_heads}")
+        q = _rows(q, "q", self.batch, heads * HEAD_DIM, self.device)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if q.shape[1] == 0:
+            return out
+        args = _lib.CacheAttentionArgs(self._view, _view(q), out.data_ptr(), q.shape[1], heads, causal, key_split)
+        _lib.launch(_lib.lib().wamffn_cache_attention, self.device.index, ctypes.byref(args))
+        return out
+
+    def status(self, clear: bool = True) -> int:
+        """Device status word (timeout / bad-index bits); synchronises the device."""
+        value = int(self._work[self.batch])
+        if clear and value:
+            self._work[self.batch:].zero_()
+        return value

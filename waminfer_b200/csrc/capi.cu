@@ -16,7 +16,10 @@
 
 #include "gemm.cuh"
 #include "attention.cuh"
+#include "kvattend.cuh"
+#include "kvcache.cuh"
 #include "pass.cuh"
+#include "rope.cuh"
 #include "rowops.cuh"
 #include "select.cuh"
 #include "wamffn.h"
@@ -163,6 +166,9 @@ int prepare_device(int device, int* sm_count) {
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(masked_attention_kernel<true, true>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     cudaFuncAttributes pass_attr{};
     WAMFFN_CUDA(cudaFuncGetAttributes(&pass_attr, stack_pass_kernel));  // its static barriers count too
     WAMFFN_CUDA(cudaFuncSetAttribute(stack_pass_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1755,6 +1761,268 @@ int wamffn_current_frame_attention(void* stream_, const wamffn_current_frame_arg
   p.batch = a->batch;
   p.status = static_cast<unsigned int*>(a->status);
   return launch_attention(stream_, maps, p, a->key_split);
+}
+
+}  // extern "C"
+
+// ================================================= norm + rotation, 8-bit cache
+namespace {
+
+// A [batch, rows, width] bf16 operand read row by row (any batch stride).
+int check_rows_view(const wamffn_rows_view& v, int64_t width, int rows, int batch, const char* name) {
+  if (!v.data) return fail(WAMFFN_ERR_INVALID, "%s is null", name);
+  if (!aligned16(v.data)) return fail(WAMFFN_ERR_INVALID, "%s must be 16-byte aligned", name);
+  if ((rows > 1 && v.row_stride < width) || v.row_stride % 8 || v.batch_stride < 0 || v.batch_stride % 8)
+    return fail(WAMFFN_ERR_INVALID, "%s strides (%lld, %lld): multiples of 8 elements, rows >= %lld apart", name,
+                (long long)v.batch_stride, (long long)v.row_stride, (long long)width);
+  return WAMFFN_OK;
+}
+
+// Launches with the programmatic-dependent-launch attribute, and in clusters along x.
+template <typename... P, typename... A>
+int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, void* stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  WAMFFN_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return WAMFFN_OK;
+}
+
+int prepare_current_device(int* sm_count) {
+  int dev = 0;
+  WAMFFN_CUDA(cudaGetDevice(&dev));
+  return prepare_device(dev, sm_count);
+}
+
+template <int D, bool kInter>
+int launch_rope(const RopeParams& p, bool whole_row, int sm, void* stream) {
+  const int heads = p.q.heads + p.k.heads;
+  const int64_t tokens = int64_t(p.batch) * p.rows;
+  if (whole_row) {
+    const int vec = heads * (D / 8);
+    const int per = vec <= 512 ? 1 : vec <= 1024 ? 2 : vec <= 2048 ? 4 : 8;
+    const int threads = ((vec + per - 1) / per + 31) / 32 * 32;
+    auto kernel = per == 1   ? rope_row_kernel<D, kInter, 1>
+                  : per == 2 ? rope_row_kernel<D, kInter, 2>
+                  : per == 4 ? rope_row_kernel<D, kInter, 4>
+                             : rope_row_kernel<D, kInter, 8>;
+    return launch_pdl(kernel, dim3(unsigned(tokens)), threads, 0, 1, stream, p);
+  }
+  constexpr int groups = kRopeThreads / (D / 8);
+  auto ctas = [&](int per) { return (tokens * ((heads + per - 1) / per) + groups - 1) / groups; };
+  if (ctas(4) > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many rows");
+  // Four heads a group read the table once for the four and keep four loads a
+  // lane in flight; while that leaves SMs idle, one head a group.
+  if (ctas(4) >= 2 * sm) return launch_pdl(rope_head_kernel<D, kInter, 4>, dim3(unsigned(ctas(4))), kRopeThreads, 0, 1, stream, p);
+  return launch_pdl(rope_head_kernel<D, kInter, 1>, dim3(unsigned(ctas(1))), kRopeThreads, 0, 1, stream, p);
+}
+
+int check_cache(const wamffn_cache_view& v, CacheView* c) {
+  if (v.blocks < 1 || v.kv_heads < 1 || v.batch < 1 || v.width < 1)
+    return fail(WAMFFN_ERR_INVALID, "cache: blocks=%d kv_heads=%d batch=%d width=%d", v.blocks, v.kv_heads, v.batch,
+                v.width);
+  if (v.kv_heads > 32767 || v.batch > 65535 || v.width > (1 << 24))
+    return fail(WAMFFN_ERR_UNSUPPORTED, "cache: kv_heads=%d batch=%d width=%d exceed the grid", v.kv_heads, v.batch,
+                v.width);
+  if (int64_t(v.blocks) * v.kv_heads > 0x7fffffff / kCacheBlock)
+    return fail(WAMFFN_ERR_UNSUPPORTED, "cache: %d blocks of %d heads exceed 2^31 rows", v.blocks, v.kv_heads);
+  if (!v.keys || !v.values || !v.key_scales || !v.value_scales || !v.block_table || !v.lengths)
+    return fail(WAMFFN_ERR_INVALID, "cache: null tensor pointer");
+  if (!aligned16(v.keys) || !aligned16(v.values)) return fail(WAMFFN_ERR_INVALID, "cache: keys and values must be 16-byte aligned");
+  if (v.batch > 1 && v.table_stride < v.width) return fail(WAMFFN_ERR_INVALID, "cache: block_table rows overlap");
+  c->keys = static_cast<uint8_t*>(v.keys);
+  c->values = static_cast<uint8_t*>(v.values);
+  c->key_scales = v.key_scales;
+  c->value_scales = v.value_scales;
+  c->table = v.block_table;
+  c->table_stride = v.table_stride;
+  c->lengths = v.lengths;
+  c->tickets = v.tickets;
+  c->status = v.status;
+  c->blocks = v.blocks;
+  c->kv_heads = v.kv_heads;
+  c->batch = v.batch;
+  c->width = v.width;
+  return WAMFFN_OK;
+}
+
+// The cache's rows as a 2-D byte tensor [blocks * kv_heads * 64, 128], box [rows, 128] with the 128-byte swizzle.
+int encode_cache(CUtensorMap* map, const void* base, const CacheView& c, int rows) {
+  auto fn = encode_fn();
+  if (!fn) return fail(WAMFFN_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[2] = {cuuint64_t(kCacheDim), cuuint64_t(c.blocks) * c.kv_heads * kCacheBlock};
+  cuuint64_t strides[1] = {cuuint64_t(kCacheDim)};
+  cuuint32_t box[2] = {cuuint32_t(kCacheDim), cuuint32_t(rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(WAMFFN_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return WAMFFN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wamffn_qk_norm_rope(void* stream, const wamffn_qk_rope_args* a) {
+  if (!a) return fail(WAMFFN_ERR_INVALID, "args is null");
+  const int d = a->head_dim;
+  if (d != 64 && d != 128 && d != 256)
+    return fail(WAMFFN_ERR_UNSUPPORTED, "head_dim=%d: 64, 128 or 256", d);
+  if (a->batch < 1 || a->rows < 1 || a->heads < 1 || a->kv_heads < 0 || a->heads > 65536 || a->kv_heads > 65536)
+    return fail(WAMFFN_ERR_INVALID, "batch=%d rows=%d heads=%d kv_heads=%d", a->batch, a->rows, a->heads, a->kv_heads);
+  if (int64_t(a->batch) * a->rows > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many rows");
+  int rc = check_rows_view(a->q, int64_t(a->heads) * d, a->rows, a->batch, "q");
+  if (rc) return rc;
+  if (a->kv_heads && (rc = check_rows_view(a->k, int64_t(a->kv_heads) * d, a->rows, a->batch, "k"))) return rc;
+  const void* ptrs[] = {a->q_weight, a->q_out, a->kv_heads ? a->k_weight : a->q_weight,
+                        a->kv_heads ? a->k_out : a->q_out};
+  for (const void* p : ptrs)
+    if (!p || !aligned16(p)) return fail(WAMFFN_ERR_INVALID, "weights and outputs must be 16-byte aligned pointers");
+  if (a->whole_row && (int64_t(a->heads) + a->kv_heads) * d > 32768)
+    return fail(WAMFFN_ERR_UNSUPPORTED, "whole-row norm: (%d + %d) heads of %d exceed 32768 elements", a->heads,
+                a->kv_heads, d);
+  RopeParams p{};
+  if (a->rope) {
+    if (a->pairs < 4 || a->pairs % 4 || a->pairs > d / 2)
+      return fail(WAMFFN_ERR_INVALID, "pairs=%d: a multiple of 4 up to %d", a->pairs, d / 2);
+    if (a->table_rows < 1 || (a->table_rows > 1 && a->table_stride < a->pairs) || a->table_stride % 2 || !aligned16(a->rope))
+      return fail(WAMFFN_ERR_INVALID, "rope table: %d rows, stride %lld (even, >= pairs), 16-byte aligned",
+                  a->table_rows, (long long)a->table_stride);
+    if (a->positions) {
+      if ((a->position_bytes != 4 && a->position_bytes != 8) ||
+          reinterpret_cast<uintptr_t>(a->positions) % a->position_bytes || a->position_stride < 0)
+        return fail(WAMFFN_ERR_INVALID, "positions: int32 or int64");
+    } else if (a->rows > a->table_rows) {
+      return fail(WAMFFN_ERR_INVALID, "%d rows and a rope table of %d", a->rows, a->table_rows);
+    }
+  }
+  int sm = 0;
+  if ((rc = prepare_current_device(&sm))) return rc;
+  p.q = RopeSide{static_cast<const __nv_bfloat16*>(a->q.data), a->q.row_stride, a->q.batch_stride,
+                 static_cast<const __nv_bfloat16*>(a->q_weight), static_cast<__nv_bfloat16*>(a->q_out), a->heads};
+  if (a->kv_heads)
+    p.k = RopeSide{static_cast<const __nv_bfloat16*>(a->k.data), a->k.row_stride, a->k.batch_stride,
+                   static_cast<const __nv_bfloat16*>(a->k_weight), static_cast<__nv_bfloat16*>(a->k_out), a->kv_heads};
+  p.rope = static_cast<const float2*>(a->rope);
+  p.table_stride = a->table_stride;
+  p.positions = a->positions;
+  p.position_stride = a->position_stride;
+  p.position_bytes = a->position_bytes;
+  p.table_rows = a->table_rows;
+  p.pairs = a->rope ? a->pairs : 0;
+  p.rows = a->rows;
+  p.batch = a->batch;
+  p.eps = a->eps;
+  const bool row = a->whole_row != 0, inter = a->interleaved != 0;
+  if (d == 64) return inter ? launch_rope<64, true>(p, row, sm, stream) : launch_rope<64, false>(p, row, sm, stream);
+  if (d == 128) return inter ? launch_rope<128, true>(p, row, sm, stream) : launch_rope<128, false>(p, row, sm, stream);
+  return inter ? launch_rope<256, true>(p, row, sm, stream) : launch_rope<256, false>(p, row, sm, stream);
+}
+
+int wamffn_cache_append(void* stream, const wamffn_cache_append_args* a) {
+  if (!a) return fail(WAMFFN_ERR_INVALID, "args is null");
+  AppendParams p{};
+  int rc = check_cache(a->cache, &p.c);
+  if (rc) return rc;
+  if (!a->cache.tickets) return fail(WAMFFN_ERR_INVALID, "cache: tickets is null");
+  if (a->rows < 1) return fail(WAMFFN_ERR_INVALID, "rows=%d", a->rows);
+  const int64_t width = int64_t(p.c.kv_heads) * kCacheDim;
+  if ((rc = check_rows_view(a->k, width, a->rows, p.c.batch, "k"))) return rc;
+  if ((rc = check_rows_view(a->v, width, a->rows, p.c.batch, "v"))) return rc;
+  int sm = 0;
+  if ((rc = prepare_current_device(&sm))) return rc;
+  p.k = static_cast<const __nv_bfloat16*>(a->k.data);
+  p.v = static_cast<const __nv_bfloat16*>(a->v.data);
+  p.k_row = a->k.row_stride;
+  p.k_batch = a->k.batch_stride;
+  p.v_row = a->v.row_stride;
+  p.v_batch = a->v.batch_stride;
+  p.counts = a->counts;
+  p.at = a->at;
+  p.rows = a->rows;
+  p.places = int(std::min<int64_t>((int64_t(a->rows) + 2 * kCacheBlock - 2) / kCacheBlock, p.c.width));
+  return launch_pdl(cache_append_kernel, dim3(unsigned(p.places), unsigned(2 * p.c.kv_heads), unsigned(p.c.batch)),
+                    kAppendThreads, 0, 1, stream, p);
+}
+
+int wamffn_cache_read(void* stream, const wamffn_cache_read_args* a) {
+  if (!a) return fail(WAMFFN_ERR_INVALID, "args is null");
+  CacheReadParams p{};
+  int rc = check_cache(a->cache, &p.c);
+  if (rc) return rc;
+  if (a->count < 1 || a->start_all < 0) return fail(WAMFFN_ERR_INVALID, "start=%d count=%d", a->start_all, a->count);
+  if (!a->k || !a->v || !aligned16(a->k) || !aligned16(a->v))
+    return fail(WAMFFN_ERR_INVALID, "k and v must be 16-byte aligned pointers");
+  int sm = 0;
+  if ((rc = prepare_current_device(&sm))) return rc;
+  p.start = a->start;
+  p.start_all = a->start_all;
+  p.count = a->count;
+  p.k = static_cast<__nv_bfloat16*>(a->k);
+  p.v = static_cast<__nv_bfloat16*>(a->v);
+  return launch_pdl(cache_read_kernel,
+                    dim3(unsigned((int64_t(a->count) + kReadRows - 1) / kReadRows), unsigned(2 * p.c.kv_heads),
+                         unsigned(p.c.batch)),
+                    kReadThreads, 0, 1, stream, p);
+}
+
+int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
+  if (!a) return fail(WAMFFN_ERR_INVALID, "args is null");
+  KvAttnParams p{};
+  int rc = check_cache(a->cache, &p.c);
+  if (rc) return rc;
+  if (a->nq < 1 || a->heads < 1 || a->heads % p.c.kv_heads)
+    return fail(WAMFFN_ERR_INVALID, "nq=%d heads=%d: heads must be a multiple of the cache's %d", a->nq, a->heads,
+                p.c.kv_heads);
+  if (a->key_split != 0 && a->key_split != 1 && a->key_split != 2 && a->key_split != 4 && a->key_split != 8)
+    return fail(WAMFFN_ERR_INVALID, "key_split=%d: 0 (automatic), 1, 2, 4 or 8", a->key_split);
+  if ((rc = check_rows_view(a->q, int64_t(a->heads) * kCacheDim, a->nq, p.c.batch, "q"))) return rc;
+  if (!a->out || !aligned16(a->out)) return fail(WAMFFN_ERR_INVALID, "out must be a 16-byte aligned pointer");
+  p.q = static_cast<const __nv_bfloat16*>(a->q.data);
+  p.q_row = a->q.row_stride;
+  p.q_batch = a->q.batch_stride;
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.nq = a->nq;
+  p.heads = a->heads;
+  p.group = a->heads / p.c.kv_heads;
+  p.causal = a->causal != 0;
+  p.scale_log2 = float((1.0 / sqrt(double(kCacheDim))) * 1.4426950408889634);
+  const int64_t rows = int64_t(a->nq) * p.group;
+  if (rows > 0x7fffffff / 16) return fail(WAMFFN_ERR_INVALID, "too many query rows");
+  int sm = 0;
+  if ((rc = prepare_current_device(&sm))) return rc;
+  const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t row_tiles = (rows + 16 * tiles - 1) / (16 * tiles);
+  // Key split: the largest that keeps the grid at two CTAs an SM and gives each key group a unit.
+  const int64_t ctas = row_tiles * p.c.kv_heads * p.c.batch;
+  const int64_t units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys);
+  p.split = 1;
+  if (a->key_split)
+    p.split = a->key_split;
+  else
+    for (int s : {2, 4, 8})
+      if (ctas * s <= 2 * sm && int64_t(s) * (kFewWarps / tiles) <= units) p.split = s;
+  if (row_tiles * p.split > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many query rows");
+  CUtensorMap kmap, vmap;
+  if ((rc = encode_cache(&kmap, p.c.keys, p.c, kUnitKeys))) return rc;
+  if ((rc = encode_cache(&vmap, p.c.values, p.c, kUnitKeys))) return rc;
+  auto kernel = tiles == 1 ? kv_attend_few_kernel<1> : tiles == 2 ? kv_attend_few_kernel<2> : kv_attend_few_kernel<4>;
+  return launch_pdl(kernel, dim3(unsigned(row_tiles * p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
+                    kFewWarps * 32, kFewSmem, p.split, stream, kmap, vmap, p);
 }
 
 }  // extern "C"

@@ -1,0 +1,457 @@
+// Attention over the 8-bit cache (kvcache.cuh):
+//
+//   out[b, i, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(q[b, i, h] . k_j / sqrt(128)),   j < seen(b, i)
+//   seen = lengths[b], or lengths[b] - nq + i + 1 (causal: the queries are the cache's last nq rows);
+//   a row that sees nothing is zeros.  heads / kv_heads query heads share a key head.
+//
+// Numbers.  k = K 2^ek and v = V 2^ev with K, V in e4m3 and one ek, ev a block
+// of 64 keys and head.  e4m3 values are exact in f16, so both products run on
+// f16 operands with fp32 sums:
+//   q is divided by a power of two of its row (largest magnitude in [1, 2)) and
+//   taken to f16: exact down to 2^-14 of the row's largest value, off by at most
+//   2^-25 of it below;
+//   x_j = (Q . K_j) 2^eq 2^ek log2(e) / sqrt(128) + ev, and the running maximum m is
+//   taken over x, so P_j = 2^(x_j - m + 14) <= 2^14 carries V's scale and never
+//   overflows f16 (full precision down to 2^-28 of the largest); P V adds up to
+//   the numerator, sum_j P_j 2^-ev (fp32, before P is rounded) to the
+//   denominator, and 2^(14 - m) cancels.
+//
+// Masked keys have x = -inf.  Rows past a sequence's length are whatever the
+// block held before; they, and NaN in a value that only some rows of a tile see,
+// must not reach the product (0 x NaN): in units where a row sees less than the
+// whole, V is cleaned, and the lowest key with a NaN in each dim is kept so that
+// the rows that do see it get it back.
+#pragma once
+
+#include "kvcache.cuh"
+#include "ptx.cuh"
+
+namespace wamffn {
+
+struct KvAttnParams {
+  CacheView c;
+  const __nv_bfloat16* q;
+  long long q_row, q_batch;  // strides, elements
+  __nv_bfloat16* out;        // [batch, nq, heads 128]
+  int nq, heads, group, causal, split;
+  float scale_log2;          // log2(e) / sqrt(128)
+};
+
+constexpr float kPBias = 14.f;
+
+__device__ __forceinline__ uint32_t f16x2_pack(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// Power of two of a query row from its largest magnitude (fp32 bits): the row is
+// multiplied by 2^-eq; infinities and NaN pass through.
+__device__ __forceinline__ int query_exp(float top) {
+  return max(-126, min(126, ((__float_as_int(top) >> 23) & 255) - 127));
+}
+
+__device__ __forceinline__ int cache_length(const CacheView& c, int b) {
+  return int(max(0ll, min((long long)c.lengths[b], (long long)c.width * kCacheBlock)));
+}
+// Keys that query token i sees.
+__device__ __forceinline__ int keys_seen(int length, int nq, int i, int causal) {
+  return causal ? max(0, length - nq + i + 1) : length;
+}
+
+// Cleans a word of 4 e4m3 values of key `key`, dims [dim, dim + 4): zero past the
+// sequence, NaN to zero with the key noted.
+__device__ __forceinline__ uint32_t clean_word(uint32_t w, int key, int length, int dim, int* nan_key, int* nan_any) {
+  if (key >= length) return 0u;
+  const uint32_t bad = __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  if (bad) {
+    for (int i = 0; i < 4; ++i)
+      if ((bad >> (8 * i)) & 1u) atomicMin(&nan_key[dim + i], key);
+    *nan_any = 1;
+  }
+  return w & ~bad;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (a decode step, the action rows): warps of 16 packed rows (query
+// token x head of the group), matrix products by mma.sync from registers.
+//
+// Bound: HBM (the cache is read once, 256 bytes a key and head).  A unit is 32
+// keys of one head, 4 KB of K and of V, loaded by TMA with the 128-byte swizzle
+// into a ring; the fragments are converted in registers (a lane takes 16
+// neighbouring dims of K, which the product's order of k allows, and the same
+// 16 dims of four rows of V), so nothing is written back to shared memory.
+// 4 warps: kTiles row tiles x (4 / kTiles) key groups with rings of their own;
+// a cluster of `split` CTAs shares the keys of a row tile, and the partial
+// results meet through distributed shared memory.
+// ---------------------------------------------------------------------------
+constexpr int kUnitKeys = 32;
+constexpr int kUnitBytes = kUnitKeys * kCacheDim;  // of K, and of V
+constexpr int kFewWarps = 4;
+constexpr int kFewStages = 12;                     // all rings together
+constexpr int kFewPitch = kCacheDim + 4;           // floats between rows of a partial result
+constexpr int kFewRing = kFewStages * 2 * kUnitBytes;
+constexpr int kFewSmem = kFewRing + 1024;
+
+template <int kTiles>
+__global__ void __launch_bounds__(kFewWarps * 32, 2)
+    kv_attend_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                         const KvAttnParams p) {
+  constexpr int kGroups = kFewWarps / kTiles;       // key groups
+  constexpr int kStages = kFewStages / kGroups;     // of a group's ring
+  constexpr int kRows = 16 * kTiles;
+  static_assert(kRows * kFewPitch * 4 <= kStages * 2 * kUnitBytes, "a partial result fits its group's ring");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full[kFewStages], empty[kFewStages];
+  __shared__ __align__(16) float2 part_ml[kGroups][kRows];  // (maximum, normaliser) of a group's rows
+  __shared__ __align__(16) float2 cta_ml[kRows];
+  __shared__ int nan_key[kCacheDim];
+  __shared__ int nan_any;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kg = warp / kTiles, mt = warp % kTiles;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = p.split, tile = int(blockIdx.x) / split, rank = int(blockIdx.x) - tile * split;
+  const int kh = blockIdx.y, b = blockIdx.z;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(smem_addr(&full[s]), 1);
+      mbar_init(smem_addr(&empty[s]), kTiles);
+    }
+    nan_any = 0;
+    abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
+  nan_key[threadIdx.x] = 0x7fffffff;  // kFewWarps * 32 == kCacheDim
+  __syncthreads();
+  pdl_wait_prior();
+  pdl_launch_dependents();
+
+  const CacheView& c = p.c;
+  const int length = cache_length(c, b);
+  const int total_rows = p.nq * p.group, row0 = tile * kRows;
+  const int rows = min(kRows, total_rows - row0);
+  const int least = keys_seen(length, p.nq, row0 / p.group, p.causal);
+  const int most = keys_seen(length, p.nq, (row0 + rows - 1) / p.group, p.causal);
+  const int units = (most + kUnitKeys - 1) / kUnitKeys;
+  const int worker = rank * kGroups + kg, workers = split * kGroups;
+  const int mine = units > worker ? (units - worker + workers - 1) / workers : 0;  // units worker + i * workers
+  uint8_t* my_ring = ring + kg * kStages * 2 * kUnitBytes;
+  uint64_t* my_full = full + kg * kStages;
+  uint64_t* my_empty = empty + kg * kStages;
+
+  // Block ids and scales of 32 of this group's units at a time, one a lane.
+  struct Info {
+    int id;     // tile row of the unit in the pool's tensor map; -1: bad block id
+    float kf;   // 2^ek
+    int ev;
+  };
+  auto info_of = [&](int i) {
+    Info f{-1, 1.f, 0};
+    if (i < mine) {
+      const int u = worker + i * workers;
+      const int id = c.table[b * c.table_stride + (u >> 1)];
+      if (id >= 0 && id < c.blocks) {
+        const size_t at = size_t(id) * c.kv_heads + kh;
+        f.id = int(at * kCacheBlock) + (u & 1) * kUnitKeys;
+        f.kf = exp2_int(scale_exp(c.key_scales[at]));
+        f.ev = scale_exp(c.value_scales[at]);
+      } else if (c.status) {
+        atomicOr(c.status, WAMFFN_DEV_BAD_INDEX);
+      }
+    }
+    return f;
+  };
+  const bool producer = mt == 0;  // this warp's lane 0 loads for the group
+  const uint64_t policy = l2_policy_evict_first();
+  Info ahead = info_of(lane);     // of the producer's chunk of 32 units
+  int ahead_chunk = 0, issued = 0;
+  auto issue = [&](int i) {  // whole warp: unit i into stage i % kStages
+    if ((i >> 5) != ahead_chunk) {
+      ahead_chunk = i >> 5;
+      ahead = info_of(ahead_chunk * 32 + lane);
+    }
+    const int id = __shfl_sync(0xffffffffu, ahead.id, i & 31);
+    if (lane == 0) {
+      const int s = i % kStages;
+      const uint32_t bar = smem_addr(&my_full[s]), dst = smem_addr(my_ring + s * 2 * kUnitBytes);
+      if (id >= 0) {
+        mbar_arrive_expect_tx(bar, 2 * kUnitBytes);
+        tma_load_2d(dst, &kmap, bar, 0, id, policy);
+        tma_load_2d(dst + kUnitBytes, &vmap, bar, 0, id, policy);
+      } else {
+        mbar_arrive_local(bar);
+      }
+    }
+    issued = i + 1;
+  };
+  if (producer)
+    for (int i = 0; i < min(mine, kStages); ++i) issue(i);
+
+  // Query fragments: rows g and g + 8 of the warp's tile, dims [32 t, 32 t + 32):
+  // step ks = 4 c + w takes dims 32 t + 16 c + 4 w + {0, 1} and {2, 3} as its k
+  // columns 2 t, 2 t + 1 and 2 t + 8, 2 t + 9.
+  uint32_t qa[8][4];
+  float qf[2];      // 2^eq log2(e) / sqrt(128) of the rows
+  int seen[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = row0 + mt * 16 + g + 8 * half;
+    const bool live = r < total_rows;
+    const int token = live ? r / p.group : 0;
+    const int head = kh * p.group + (live ? r - token * p.group : 0);
+    seen[half] = live ? keys_seen(length, p.nq, token, p.causal) : 0;
+    const __nv_bfloat16* src = p.q + b * p.q_batch + token * p.q_row + size_t(head) * kCacheDim + 32 * t;
+    uint4 u[4];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] = live ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(bf2_lo(w[e])), fabsf(bf2_hi(w[e]))));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int eq = query_exp(top);
+    const float inv = exp2_int(-eq);
+    qf[half] = exp2_int(eq) * p.scale_log2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)  // words 4 i + e: dims 32 t + 8 i + 2 e; step 2 i + e / 2, column pair e % 2
+        qa[2 * i + (e >> 1)][half + 2 * (e & 1)] = f16x2_pack(bf2_lo(w[e]) * inv, bf2_hi(w[e]) * inv);
+    }
+  }
+
+  float o[16][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  Info now = ahead;
+  int now_chunk = 0;
+  bool ok = true;
+  for (int i = 0; i < mine; ++i) {
+    const int s = i % kStages;
+    if (producer && i > 0 && i - 1 + kStages < mine) {  // refill the stage of the previous unit
+      if (kTiles > 1)
+        ok = wait_bounded(smem_addr(&my_empty[(i - 1) % kStages]), uint32_t((i - 1) / kStages) & 1u, &abort_flag,
+                          c.status, WAMFFN_DEV_TIMEOUT);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      issue(i - 1 + kStages);
+    }
+    if ((i >> 5) != now_chunk) {
+      now_chunk = i >> 5;
+      now = info_of(now_chunk * 32 + lane);
+    }
+    const int id = __shfl_sync(0xffffffffu, now.id, i & 31);
+    const float kf = __shfl_sync(0xffffffffu, now.kf, i & 31);
+    const int ev = __shfl_sync(0xffffffffu, now.ev, i & 31);
+    ok = wait_bounded(smem_addr(&my_full[s]), uint32_t(i / kStages) & 1u, &abort_flag, c.status, WAMFFN_DEV_TIMEOUT);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    if (id >= 0) {
+      const int key0 = (worker + i * workers) * kUnitKeys;
+      const uint32_t kb = smem_addr(my_ring + s * 2 * kUnitBytes), vb = kb + kUnitBytes;
+      // S = Q K^T, 8 keys a tile.
+      float x[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
+        const uint32_t row = kb + (nt * 8 + g) * kCacheDim;
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const uint4 u = lds128(row + (((2 * t + cc) ^ g) << 4));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            mma_f16(x[nt], qa[cc * 4 + e], e4m3x2_to_f16x2(w[e]), e4m3x2_hi_to_f16x2(w[e]));
+        }
+      }
+      const bool whole = key0 + kUnitKeys <= least;  // every row of the tile sees every key of the unit
+      const float f0 = qf[0] * kf, f1 = qf[1] * kf, evf = float(ev);
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = fmaf(x[nt][e], (e >> 1) ? f1 : f0, evf);
+          if (!whole && key0 + nt * 8 + 2 * t + (e & 1) >= seen[e >> 1]) v = -INFINITY;
+          x[nt][e] = v;
+          top[e >> 1] = fmaxf(top[e >> 1], v);
+        }
+      float base[2], corr[2];
+      bool grown = false;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+        const float next = fmaxf(m[half], top[half]);
+        const float safe = next == -INFINITY ? 0.f : next;
+        corr[half] = ex2_approx(m[half] - safe);
+        grown |= next != m[half];
+        m[half] = next;
+        base[half] = kPBias - safe;
+      }
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[nt][e] = ex2_approx(x[nt][e] + base[e >> 1]);
+          sum[e >> 1] += x[nt][e];
+        }
+      const float back = exp2_int(-ev);
+      l[0] = fmaf(sum[0], back, l[0] * corr[0]);
+      l[1] = fmaf(sum[1], back, l[1] * corr[1]);
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          o[n][0] *= corr[0], o[n][1] *= corr[0];
+          o[n][2] *= corr[1], o[n][3] *= corr[1];
+        }
+      }
+      // O += P V, 16 keys a step; tile n holds dims 16 g' + n (g' the tile's column).
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint32_t pa[4] = {f16x2_pack(x[2 * ks][0], x[2 * ks][1]), f16x2_pack(x[2 * ks][2], x[2 * ks][3]),
+                                f16x2_pack(x[2 * ks + 1][0], x[2 * ks + 1][1]),
+                                f16x2_pack(x[2 * ks + 1][2], x[2 * ks + 1][3])};
+        uint32_t w[4][4];  // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the step, dims [16 g, 16 g + 16)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = ks * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
+          const uint4 u = lds128(vb + row * kCacheDim + ((g ^ (2 * t + (r & 1))) << 4));
+          w[r][0] = u.x, w[r][1] = u.y, w[r][2] = u.z, w[r][3] = u.w;
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[r][e] = clean_word(w[r][e], key0 + row, length, 16 * g + 4 * e, nan_key, &nan_any);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = __byte_perm(w[0][e], w[1][e], 0x5140), z = __byte_perm(w[2][e], w[3][e], 0x5140);
+          const uint32_t a2 = __byte_perm(w[0][e], w[1][e], 0x7362), z2 = __byte_perm(w[2][e], w[3][e], 0x7362);
+          mma_f16(o[4 * e], pa, e4m3x2_to_f16x2(a), e4m3x2_to_f16x2(z));
+          mma_f16(o[4 * e + 1], pa, e4m3x2_hi_to_f16x2(a), e4m3x2_hi_to_f16x2(z));
+          mma_f16(o[4 * e + 2], pa, e4m3x2_to_f16x2(a2), e4m3x2_to_f16x2(z2));
+          mma_f16(o[4 * e + 3], pa, e4m3x2_hi_to_f16x2(a2), e4m3x2_hi_to_f16x2(z2));
+        }
+      }
+    }
+    __syncwarp();
+    if (kTiles > 1 && lane == 0) mbar_arrive_local(smem_addr(&my_empty[s]));
+  }
+  if (!ok && producer && lane == 0)  // copies in flight land before the shared memory is given up
+    for (int i = max(0, issued - kStages); i < issued; ++i)
+      wait_drain(smem_addr(&my_full[i % kStages]), uint32_t(i / kStages) & 1u);
+  __syncthreads();  // every ring is idle: partial results go over them
+  float* part = reinterpret_cast<float*>(my_ring);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+    l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+    const int r = mt * 16 + g + 8 * half;
+    if (t == 0) part_ml[kg][r] = make_float2(m[half], l[half]);
+#pragma unroll
+    for (int n = 0; n < 16; n += 4)
+#pragma unroll
+      for (int col = 0; col < 2; ++col) {  // column 2 t + col of tiles n .. n + 3: dims 32 t + 16 col + n
+        const int dim = 32 * t + 16 * col + n;
+        float4 v = make_float4(o[n][2 * half + col], o[n + 1][2 * half + col], o[n + 2][2 * half + col],
+                               o[n + 3][2 * half + col]);
+        if (nan_any) {
+          const float bad = __int_as_float(0x7fffffff);
+          if (nan_key[dim] < seen[half]) v.x = bad;
+          if (nan_key[dim + 1] < seen[half]) v.y = bad;
+          if (nan_key[dim + 2] < seen[half]) v.z = bad;
+          if (nan_key[dim + 3] < seen[half]) v.w = bad;
+        }
+        *reinterpret_cast<float4*>(part + r * kFewPitch + dim) = v;
+      }
+  }
+  __syncthreads();
+  // The groups' partial results into group 0's place.
+  for (int i = threadIdx.x; i < rows * (kCacheDim / 4); i += kFewWarps * 32) {
+    const int r = i >> 5, d = (i & 31) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) top = fmaxf(top, part_ml[k][r].x);
+    const float safe = top == -INFINITY ? 0.f : top;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const float f = ex2_approx(part_ml[k][r].x - safe);
+      const float4 u = *reinterpret_cast<const float4*>(
+          reinterpret_cast<const float*>(ring + k * kStages * 2 * kUnitBytes) + r * kFewPitch + d);
+      v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+      sum += part_ml[k][r].y * f;
+    }
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(ring) + r * kFewPitch + d) = v;
+    if (d == 0) cta_ml[r] = make_float2(top, sum);
+  }
+  if (split > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  // The cluster's partial results, in rank order; rank r takes every split-th 4-dim piece.
+  for (int i = rank + split * int(threadIdx.x); i < rows * (kCacheDim / 4); i += split * kFewWarps * 32) {
+    const int r = i >> 5, d = (i & 31) * 4;
+    const uint32_t ml_at = smem_addr(&cta_ml[r]), o_at = smem_addr(reinterpret_cast<float*>(ring) + r * kFewPitch + d);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.f;
+    for (int k = 0; k < split; ++k) {  // running maximum: one pass over the peers
+      const float2 ml = split > 1 ? ld_cluster2(map_to_cta(ml_at, k)) : cta_ml[r];
+      const float4 u = split > 1 ? ld_cluster4(map_to_cta(o_at, k))
+                                 : *reinterpret_cast<const float4*>(reinterpret_cast<float*>(ring) + r * kFewPitch + d);
+      const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
+      const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
+      v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
+      v.z = v.z * fo + u.z * fn, v.w = v.w * fo + u.w * fn;
+      sum = sum * fo + ml.y * fn;
+      top = next;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // nothing seen: zeros
+    const int row = row0 + r, token = row / p.group, head = kh * p.group + row - token * p.group;
+    if (!abort_flag)
+      *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.nq + token) * p.heads + head) * kCacheDim + d) =
+          make_uint2(bf2_pack(v.x * inv, v.y * inv), bf2_pack(v.z * inv, v.w * inv));
+  }
+  if (split > 1) cluster_sync();  // no CTA leaves while a peer reads its shared memory
+}
+
+}  // namespace wamffn
