@@ -17,6 +17,7 @@
 #include "gemm.cuh"
 #include "attention.cuh"
 #include "kvattend.cuh"
+#include "kvattend_many.cuh"
 #include "kvcache.cuh"
 #include "pass.cuh"
 #include "rope.cuh"
@@ -169,6 +170,13 @@ int prepare_device(int device, int* sm_count) {
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
+    // The kernel's warpgroups trade registers: the launch must bring what they share out.
+    cudaFuncAttributes many_attr{};
+    WAMFFN_CUDA(cudaFuncGetAttributes(&many_attr, kv_attend_many_kernel));
+    if (many_attr.numRegs != kManyLaunchRegs)
+      return fail(WAMFFN_ERR_UNSUPPORTED, "kv_attend_many_kernel has %d registers, not %d", many_attr.numRegs,
+                  kManyLaunchRegs);
     cudaFuncAttributes pass_attr{};
     WAMFFN_CUDA(cudaFuncGetAttributes(&pass_attr, stack_pass_kernel));  // its static barriers count too
     WAMFFN_CUDA(cudaFuncSetAttribute(stack_pass_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1829,6 +1837,28 @@ int launch_rope(const RopeParams& p, bool whole_row, int sm, void* stream) {
   return launch_pdl(rope_head_kernel<D, kInter, 1>, dim3(unsigned(ctas(1))), kRopeThreads, 0, 1, stream, p);
 }
 
+// Clusters of `split` CTAs of kv_attend_many_kernel that the current device holds at once.
+int64_t many_clusters(int split) {
+  static std::atomic<int> known[64][9];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if ((n = known[dev][split].load(std::memory_order_relaxed)) > 0) return n;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(split));
+  cfg.blockDim = dim3(kManyThreads);
+  cfg.dynamicSmemBytes = kManySmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kv_attend_many_kernel, &cfg) != cudaSuccess) return 0;
+  known[dev][split].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 int check_cache(const wamffn_cache_view& v, CacheView* c) {
   if (v.blocks < 1 || v.kv_heads < 1 || v.batch < 1 || v.width < 1)
     return fail(WAMFFN_ERR_INVALID, "cache: blocks=%d kv_heads=%d batch=%d width=%d", v.blocks, v.kv_heads, v.batch,
@@ -2005,6 +2035,18 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   if (rows > 0x7fffffff / 16) return fail(WAMFFN_ERR_INVALID, "too many query rows");
   int sm = 0;
   if ((rc = prepare_current_device(&sm))) return rc;
+  if (rows > kFewMaxRows) {
+    const int64_t row_tiles = (rows + kManyRows - 1) / kManyRows, ctas = row_tiles * p.c.kv_heads * p.c.batch;
+    // Key split: the largest that keeps the grid within one wave (a CTA fills an SM) and leaves each CTA two steps.
+    const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
+    p.split = a->key_split ? a->key_split : 1;
+    if (!a->key_split)
+      for (int s = 2; s <= 8; ++s)
+        if (ctas <= many_clusters(s) && 2 * s <= steps) p.split = s;
+    if (row_tiles * p.split > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many query rows");
+    return launch_pdl(kv_attend_many_kernel, dim3(unsigned(row_tiles * p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
+                      kManyThreads, kManySmem, p.split, stream, p);
+  }
   const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int64_t row_tiles = (rows + 16 * tiles - 1) / (16 * tiles);
   // Key split: the largest that keeps the grid at two CTAs an SM and gives each key group a unit.
@@ -2016,7 +2058,6 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   else
     for (int s : {2, 4, 8})
       if (ctas * s <= 2 * sm && int64_t(s) * (kFewWarps / tiles) <= units) p.split = s;
-  if (row_tiles * p.split > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many query rows");
   CUtensorMap kmap, vmap;
   if ((rc = encode_cache(&kmap, p.c.keys, p.c, kUnitKeys))) return rc;
   if ((rc = encode_cache(&vmap, p.c.values, p.c, kUnitKeys))) return rc;

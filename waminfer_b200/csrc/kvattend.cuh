@@ -72,9 +72,10 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
 }
 
 // Power of two of a query row from its largest magnitude (fp32 bits): the row is
-// multiplied by 2^-eq; infinities and NaN pass through.
+// multiplied by 2^-eq; infinities and NaN pass through.  At least -60, so that
+// 2^eq 2^ek / sqrt(128) stays a normal number (-inf times it is -inf).
 __device__ __forceinline__ int query_exp(float top) {
-  return max(-126, min(126, ((__float_as_int(top) >> 23) & 255) - 127));
+  return max(-60, min(126, ((__float_as_int(top) >> 23) & 255) - 127));
 }
 
 __device__ __forceinline__ int cache_length(const CacheView& c, int b) {
@@ -111,6 +112,7 @@ __device__ __forceinline__ uint32_t clean_word(uint32_t w, int key, int length, 
 // a cluster of `split` CTAs shares the keys of a row tile, and the partial
 // results meet through distributed shared memory.
 // ---------------------------------------------------------------------------
+constexpr int kFewMaxRows = 64;  // packed rows of a key head; beyond, kvattend_many.cuh
 constexpr int kUnitKeys = 32;
 constexpr int kUnitBytes = kUnitKeys * kCacheDim;  // of K, and of V
 constexpr int kFewWarps = 4;
