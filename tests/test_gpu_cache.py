@@ -297,6 +297,28 @@ def test_attend_key_split(cuda_device, split, nq, heads, kv_heads, lengths):
     close(cache.attend(q, heads, causal=True, key_split=split), attention(Model(cache), q, heads, True), max(lengths))
 
 
+@pytest.mark.parametrize("nq,heads,kv_heads,lengths,causal", [
+    (257, 8, 1, [1111], True), (130, 4, 4, [3000, 900], False), (300, 16, 2, [2000], True), (2, 8, 2, [5000, 3], True),
+    (9, 6, 2, [777, 64], False), (60, 3, 3, [1500], True)])
+def test_attend_gives_the_same_bits_again(cuda_device, nq, heads, kv_heads, lengths, causal):
+    """Steps, stages and partial results meet in a fixed order: forty runs back to back, one result."""
+    cache, g = make(cuda_device, nq, len(lengths), kv_heads, lengths, spread=3)
+    q = rows(g, len(lengths), nq, heads * DIM)
+    runs = [cache.attend(q, heads, causal=causal) for _ in range(40)]
+    assert all(torch.equal(runs[0], r) for r in runs[1:])
+    close(runs[0], attention(Model(cache), q, heads, causal), max(lengths))
+
+
+@pytest.mark.parametrize("nq", [1, 70])
+def test_attend_zero_queries_over_the_smallest_scales(cuda_device, nq):
+    """A row of zeros over keys of the least scale: masked keys stay masked, the values' mean comes out."""
+    cache, g = make(cuda_device, nq, 1, 2, [70], spread=1)
+    cache.key_scales.fill_(2.0 ** -60)
+    q = torch.zeros(1, nq, 256, dtype=torch.bfloat16, device=cuda_device)
+    for causal in (False, True):
+        close(cache.attend(q, 2, causal=causal), attention(Model(cache), q, 2, causal), 70)
+
+
 @pytest.mark.parametrize("nq", [1, 20, 200])
 def test_attend_scales_far_apart(cuda_device, nq):
     """Values of one block 2^40 times another's, a block of zeros, queries of very different sizes and sharp scores."""

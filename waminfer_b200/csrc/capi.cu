@@ -171,12 +171,6 @@ int prepare_device(int device, int* sm_count) {
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
-    // The kernel's warpgroups trade registers: the launch must bring what they share out.
-    cudaFuncAttributes many_attr{};
-    WAMFFN_CUDA(cudaFuncGetAttributes(&many_attr, kv_attend_many_kernel));
-    if (many_attr.numRegs != kManyLaunchRegs)
-      return fail(WAMFFN_ERR_UNSUPPORTED, "kv_attend_many_kernel has %d registers, not %d", many_attr.numRegs,
-                  kManyLaunchRegs);
     cudaFuncAttributes pass_attr{};
     WAMFFN_CUDA(cudaFuncGetAttributes(&pass_attr, stack_pass_kernel));  // its static barriers count too
     WAMFFN_CUDA(cudaFuncSetAttribute(stack_pass_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -2037,12 +2031,19 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   if ((rc = prepare_current_device(&sm))) return rc;
   if (rows > kFewMaxRows) {
     const int64_t row_tiles = (rows + kManyRows - 1) / kManyRows, ctas = row_tiles * p.c.kv_heads * p.c.batch;
-    // Key split: the largest that keeps the grid within one wave (a CTA fills an SM) and leaves each CTA two steps.
+    // Key split: the one with the least waves x (steps of a CTA + what a CTA costs besides, about four steps);
+    // clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
     const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
     p.split = a->key_split ? a->key_split : 1;
-    if (!a->key_split)
-      for (int s = 2; s <= 8; ++s)
-        if (ctas <= many_clusters(s) && 2 * s <= steps) p.split = s;
+    if (!a->key_split) {
+      int64_t best = 0;
+      for (int s = 1; s <= 8 && 2 * s <= std::max<int64_t>(steps, 2); ++s) {
+        const int64_t at_once = s == 1 ? sm : many_clusters(s);
+        if (at_once < 1) continue;
+        const int64_t cost = (ctas + at_once - 1) / at_once * ((steps + s - 1) / s + 4);
+        if (best == 0 || cost < best) best = cost, p.split = s;
+      }
+    }
     if (row_tiles * p.split > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many query rows");
     return launch_pdl(kv_attend_many_kernel, dim3(unsigned(row_tiles * p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
                       kManyThreads, kManySmem, p.split, stream, p);

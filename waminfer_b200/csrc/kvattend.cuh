@@ -57,6 +57,9 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -86,17 +89,21 @@ __device__ __forceinline__ int keys_seen(int length, int nq, int i, int causal) 
   return causal ? max(0, length - nq + i + 1) : length;
 }
 
-// Cleans a word of 4 e4m3 values of key `key`, dims [dim, dim + 4): zero past the
+// Cleans 16 e4m3 values, dims [dim, dim + 16) of key `key`: zero past the
 // sequence, NaN to zero with the key noted.
-__device__ __forceinline__ uint32_t clean_word(uint32_t w, int key, int length, int dim, int* nan_key, int* nan_any) {
-  if (key >= length) return 0u;
-  const uint32_t bad = __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
-  if (bad) {
-    for (int i = 0; i < 4; ++i)
-      if ((bad >> (8 * i)) & 1u) atomicMin(&nan_key[dim + i], key);
-    *nan_any = 1;
+__device__ __noinline__ uint4 clean_chunk(uint4 u, int key, int length, int dim, int* nan_key, int* nan_any) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t byte = (w[i >> 2] >> (8 * (i & 3))) & 0x7fu;
+    if (key < length && byte == 0x7fu) {
+      atomicMin(&nan_key[dim + i], key);
+      *nan_any = 1;
+    }
   }
-  return w & ~bad;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = key < length ? w[e] & ~__vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu) : 0u;
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---------------------------------------------------------------------------
@@ -303,6 +310,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         }
       }
       const bool whole = key0 + kUnitKeys <= least;  // every row of the tile sees every key of the unit
+      if (!whole) {
+        // Each warp that reads the unit cleans all of it: the warps of a group write the same values.
+#pragma unroll 1
+        for (int e = lane; e < kUnitKeys * 8; e += 32) {
+          const int row = e >> 3, chunk = e & 7;
+          const uint32_t at = vb + row * kCacheDim + (chunk << 4);
+          sts128(at, clean_chunk(lds128(at), key0 + row, length, 16 * (chunk ^ (row & 7)), nan_key, &nan_any));
+        }
+        fence_proxy_async();  // the place is refilled by a bulk copy
+        __syncwarp();
+      }
       const float f0 = qf[0] * kf, f1 = qf[1] * kf, evf = float(ev);
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -357,11 +375,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
           const int row = ks * 16 + 2 * t + (r & 1) + 8 * (r >> 1);
           const uint4 u = lds128(vb + row * kCacheDim + ((g ^ (2 * t + (r & 1))) << 4));
           w[r][0] = u.x, w[r][1] = u.y, w[r][2] = u.z, w[r][3] = u.w;
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[r][e] = clean_word(w[r][e], key0 + row, length, 16 * g + 4 * e, nan_key, &nan_any);
-          }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
