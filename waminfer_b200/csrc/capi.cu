@@ -2050,15 +2050,16 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   }
   const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int64_t row_tiles = (rows + 16 * tiles - 1) / (16 * tiles);
-  // Key split: the largest that keeps the grid at two CTAs an SM and gives each key group a unit.
+  // Key split: enough CTAs for two an SM, as long as a key group has a unit; and beyond that as long as it has
+  // sixteen, so that ragged sequences even out over several waves.
   const int64_t ctas = row_tiles * p.c.kv_heads * p.c.batch;
-  const int64_t units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys);
+  const int64_t units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys), groups = kFewWarps / tiles;
   p.split = 1;
   if (a->key_split)
     p.split = a->key_split;
   else
     for (int s : {2, 4, 8})
-      if (ctas * s <= 2 * sm && int64_t(s) * (kFewWarps / tiles) <= units) p.split = s;
+      if (s * groups * 16 <= units || (ctas * s <= 2 * sm && s * groups <= units)) p.split = s;
   CUtensorMap kmap, vmap;
   if ((rc = encode_cache(&kmap, p.c.keys, p.c, kUnitKeys))) return rc;
   if ((rc = encode_cache(&vmap, p.c.values, p.c, kUnitKeys))) return rc;

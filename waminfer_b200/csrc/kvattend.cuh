@@ -89,21 +89,34 @@ __device__ __forceinline__ int keys_seen(int length, int nq, int i, int causal) 
   return causal ? max(0, length - nq + i + 1) : length;
 }
 
-// Cleans 16 e4m3 values, dims [dim, dim + 16) of key `key`: zero past the
-// sequence, NaN to zero with the key noted.
-__device__ __noinline__ uint4 clean_chunk(uint4 u, int key, int length, int dim, int* nan_key, int* nan_any) {
+// Whether one of 16 e4m3 values is NaN (a byte is 0x7f but for its sign).
+__device__ __forceinline__ bool any_nan(const uint4& u) {
+  const uint32_t x = (u.x & 0x7f7f7f7fu) + 0x01010101u, y = (u.y & 0x7f7f7f7fu) + 0x01010101u,
+                 z = (u.z & 0x7f7f7f7fu) + 0x01010101u, w = (u.w & 0x7f7f7f7fu) + 0x01010101u;
+  return ((x | y | z | w) & 0x80808080u) != 0;
+}
+// 16 e4m3 values, dims [dim, dim + 16) of key `key`, without their NaN, whose key is noted (rare).
+__device__ __noinline__ uint4 drop_nan(uint4 u, int key, int dim, int* nan_key, int* nan_any) {
   uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll 1
   for (int i = 0; i < 16; ++i) {
-    const uint32_t byte = (w[i >> 2] >> (8 * (i & 3))) & 0x7fu;
-    if (key < length && byte == 0x7fu) {
+    const uint32_t at = 8 * (i & 3), word = i < 8 ? (i < 4 ? w[0] : w[1]) : (i < 12 ? w[2] : w[3]);
+    if (((word >> at) & 0x7fu) == 0x7fu) {
       atomicMin(&nan_key[dim + i], key);
       *nan_any = 1;
     }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = key < length ? w[e] & ~__vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu) : 0u;
+  for (int e = 0; e < 4; ++e) w[e] &= ~__vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// What the product may see of 16 values: nothing past the sequence; no NaN in a
+// unit that some rows see less of than others (`scan`).
+__device__ __forceinline__ uint4 clean_chunk(uint4 u, int key, int length, bool scan, int dim, int* nan_key,
+                                             int* nan_any) {
+  if (key >= length) return make_uint4(0, 0, 0, 0);
+  if (scan && any_nan(u)) u = drop_nan(u, key, dim, nan_key, nan_any);
+  return u;
 }
 
 // ---------------------------------------------------------------------------
@@ -168,48 +181,47 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   pdl_launch_dependents();
 
   const CacheView& c = p.c;
+  const int worker = rank * kGroups + kg, workers = split * kGroups;
+  uint8_t* my_ring = ring + kg * kStages * 2 * kUnitBytes;
+  uint64_t* my_full = full + kg * kStages;
+  uint64_t* my_empty = empty + kg * kStages;
+  // Block ids and scales of 32 of this group's units (worker + i * workers) at a time, one a lane.  The scales are
+  // taken apart where they are used: no load waits for them.
+  struct Info {
+    int id;         // tile row of the unit in the pool's tensor map; -1: bad block id
+    float ks, vs;
+  };
+  auto table_at = [&](int i) {  // any entry of the table, whatever the length
+    const int at = (worker + i * workers) >> 1;
+    return at < c.width ? c.table[b * c.table_stride + at] : -1;
+  };
+  auto info_of = [&](int i, int id) {
+    Info f{-1, 1.f, 1.f};
+    if (id >= 0 && id < c.blocks) {
+      const size_t at = size_t(id) * c.kv_heads + kh;
+      f.id = int(at * kCacheBlock) + ((worker + i * workers) & 1) * kUnitKeys;
+      f.ks = c.key_scales[at];
+      f.vs = c.value_scales[at];
+    }
+    return f;
+  };
+  const int first_id = table_at(lane);  // on its way together with the length
   const int length = cache_length(c, b);
   const int total_rows = p.nq * p.group, row0 = tile * kRows;
   const int rows = min(kRows, total_rows - row0);
   const int least = keys_seen(length, p.nq, row0 / p.group, p.causal);
   const int most = keys_seen(length, p.nq, (row0 + rows - 1) / p.group, p.causal);
   const int units = (most + kUnitKeys - 1) / kUnitKeys;
-  const int worker = rank * kGroups + kg, workers = split * kGroups;
-  const int mine = units > worker ? (units - worker + workers - 1) / workers : 0;  // units worker + i * workers
-  uint8_t* my_ring = ring + kg * kStages * 2 * kUnitBytes;
-  uint64_t* my_full = full + kg * kStages;
-  uint64_t* my_empty = empty + kg * kStages;
+  const int mine = units > worker ? (units - worker + workers - 1) / workers : 0;
 
-  // Block ids and scales of 32 of this group's units at a time, one a lane.
-  struct Info {
-    int id;     // tile row of the unit in the pool's tensor map; -1: bad block id
-    float kf;   // 2^ek
-    int ev;
-  };
-  auto info_of = [&](int i) {
-    Info f{-1, 1.f, 0};
-    if (i < mine) {
-      const int u = worker + i * workers;
-      const int id = c.table[b * c.table_stride + (u >> 1)];
-      if (id >= 0 && id < c.blocks) {
-        const size_t at = size_t(id) * c.kv_heads + kh;
-        f.id = int(at * kCacheBlock) + (u & 1) * kUnitKeys;
-        f.kf = exp2_int(scale_exp(c.key_scales[at]));
-        f.ev = scale_exp(c.value_scales[at]);
-      } else if (c.status) {
-        atomicOr(c.status, WAMFFN_DEV_BAD_INDEX);
-      }
-    }
-    return f;
-  };
   const bool producer = mt == 0;  // this warp's lane 0 loads for the group
   const uint64_t policy = l2_policy_evict_first();
-  Info ahead = info_of(lane);     // of the producer's chunk of 32 units
+  Info ahead = info_of(lane, first_id);  // of the producer's chunk of 32 units
   int ahead_chunk = 0, issued = 0;
   auto issue = [&](int i) {  // whole warp: unit i into stage i % kStages
     if ((i >> 5) != ahead_chunk) {
       ahead_chunk = i >> 5;
-      ahead = info_of(ahead_chunk * 32 + lane);
+      ahead = info_of(ahead_chunk * 32 + lane, table_at(ahead_chunk * 32 + lane));
     }
     const int id = __shfl_sync(0xffffffffu, ahead.id, i & 31);
     if (lane == 0) {
@@ -221,6 +233,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         tma_load_2d(dst + kUnitBytes, &vmap, bar, 0, id, policy);
       } else {
         mbar_arrive_local(bar);
+        if (c.status) atomicOr(c.status, WAMFFN_DEV_BAD_INDEX);
       }
     }
     issued = i + 1;
@@ -282,41 +295,43 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     }
     if ((i >> 5) != now_chunk) {
       now_chunk = i >> 5;
-      now = info_of(now_chunk * 32 + lane);
+      now = info_of(now_chunk * 32 + lane, table_at(now_chunk * 32 + lane));
     }
     const int id = __shfl_sync(0xffffffffu, now.id, i & 31);
-    const float kf = __shfl_sync(0xffffffffu, now.kf, i & 31);
-    const int ev = __shfl_sync(0xffffffffu, now.ev, i & 31);
+    const float kf = exp2_int(scale_exp(__shfl_sync(0xffffffffu, now.ks, i & 31)));
+    const int ev = scale_exp(__shfl_sync(0xffffffffu, now.vs, i & 31));
     ok = wait_bounded(smem_addr(&my_full[s]), uint32_t(i / kStages) & 1u, &abort_flag, c.status, WAMFFN_DEV_TIMEOUT);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     if (id >= 0) {
       const int key0 = (worker + i * workers) * kUnitKeys;
       const uint32_t kb = smem_addr(my_ring + s * 2 * kUnitBytes), vb = kb + kUnitBytes;
-      // S = Q K^T, 8 keys a tile.
-      float x[4][4];
+      // S = Q K^T, 8 keys a tile; the four tiles' sums advance together.
+      float x[4][4] = {};
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
+      for (int cc = 0; cc < 2; ++cc) {
+        uint32_t w[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
-        const uint32_t row = kb + (nt * 8 + g) * kCacheDim;
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const uint4 u = lds128(row + (((2 * t + cc) ^ g) << 4));
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mma_f16(x[nt], qa[cc * 4 + e], e4m3x2_to_f16x2(w[e]), e4m3x2_hi_to_f16x2(w[e]));
+        for (int nt = 0; nt < 4; ++nt) {
+          const uint4 u = lds128(kb + (nt * 8 + g) * kCacheDim + (((2 * t + cc) ^ g) << 4));
+          w[nt][0] = u.x, w[nt][1] = u.y, w[nt][2] = u.z, w[nt][3] = u.w;
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt)
+            mma_f16(x[nt], qa[cc * 4 + e], e4m3x2_to_f16x2(w[nt][e]), e4m3x2_hi_to_f16x2(w[nt][e]));
       }
       const bool whole = key0 + kUnitKeys <= least;  // every row of the tile sees every key of the unit
       if (!whole) {
-        // Each warp that reads the unit cleans all of it: the warps of a group write the same values.
+        // Each warp that reads the unit cleans all of it: the warps of a group write the same values.  Rows that
+        // every row of the tile sees need no look.
 #pragma unroll 1
-        for (int e = lane; e < kUnitKeys * 8; e += 32) {
+        for (int e = max(0, (least < most ? least : length) - key0) * 8 + lane; e < kUnitKeys * 8; e += 32) {
           const int row = e >> 3, chunk = e & 7;
           const uint32_t at = vb + row * kCacheDim + (chunk << 4);
-          sts128(at, clean_chunk(lds128(at), key0 + row, length, 16 * (chunk ^ (row & 7)), nan_key, &nan_any));
+          sts128(at, clean_chunk(lds128(at), key0 + row, length, least < most, 16 * (chunk ^ (row & 7)), nan_key,
+                                 &nan_any));
         }
         fence_proxy_async();  // the place is refilled by a bulk copy
         __syncwarp();
@@ -447,18 +462,29 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   for (int i = rank + split * int(threadIdx.x); i < rows * (kCacheDim / 4); i += split * kFewWarps * 32) {
     const int r = i >> 5, d = (i & 31) * 4;
     const uint32_t ml_at = smem_addr(&cta_ml[r]), o_at = smem_addr(reinterpret_cast<float*>(ring) + r * kFewPitch + d);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u[8];
+    float2 ml[8];
     float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < split; ++k) {  // running maximum: one pass over the peers
-      const float2 ml = split > 1 ? ld_cluster2(map_to_cta(ml_at, k)) : cta_ml[r];
-      const float4 u = split > 1 ? ld_cluster4(map_to_cta(o_at, k))
-                                 : *reinterpret_cast<const float4*>(reinterpret_cast<float*>(ring) + r * kFewPitch + d);
-      const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
-      const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
-      v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
-      v.z = v.z * fo + u.z * fn, v.w = v.w * fo + u.w * fn;
-      sum = sum * fo + ml.y * fn;
-      top = next;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {  // all peers' loads before the first use
+      ml[k] = make_float2(-INFINITY, 0.f);
+      u[k] = v;
+      if (split == 1 && k == 0) {
+        ml[k] = cta_ml[r];
+        u[k] = *reinterpret_cast<float4*>(reinterpret_cast<float*>(ring) + r * kFewPitch + d);
+      } else if (k < split) {
+        ml[k] = ld_cluster2(map_to_cta(ml_at, k));
+        u[k] = ld_cluster4(map_to_cta(o_at, k));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+    const float safe = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = ex2_approx(ml[k].x - safe);
+      v.x += u[k].x * f, v.y += u[k].y * f, v.z += u[k].z * f, v.w += u[k].w * f;
+      sum += ml[k].y * f;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // nothing seen: zeros
     const int row = row0 + r, token = row / p.group, head = kh * p.group + row - token * p.group;

@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       if (key0 + kManyStep > least) {  // some row sees less than the whole step
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          r.v[i] = clean_chunk(r.v[i], key0 + r0 + 16 * i, length, 16 * chunk, sh.nan_key, &sh.nan_any);
+          r.v[i] = clean_chunk(r.v[i], key0 + r0 + 16 * i, length, least < most, 16 * chunk, sh.nan_key, &sh.nan_any);
       }
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
