@@ -171,6 +171,12 @@ int prepare_device(int device, int* sm_count) {
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
+    // The kernel's warpgroups trade registers: a split that the launch does not bring would wait for good.
+    cudaFuncAttributes many_attr{};
+    WAMFFN_CUDA(cudaFuncGetAttributes(&many_attr, kv_attend_many_kernel));
+    if (many_attr.numRegs != kManyLaunchRegs)
+      return fail(WAMFFN_ERR_UNSUPPORTED, "kv_attend_many_kernel has %d registers, not %d", many_attr.numRegs,
+                  kManyLaunchRegs);
     cudaFuncAttributes pass_attr{};
     WAMFFN_CUDA(cudaFuncGetAttributes(&pass_attr, stack_pass_kernel));  // its static barriers count too
     WAMFFN_CUDA(cudaFuncSetAttribute(stack_pass_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -11,10 +11,11 @@
 //   taken to f16: exact down to 2^-14 of the row's largest value, off by at most
 //   2^-25 of it below;
 //   x_j = (Q . K_j) 2^eq 2^ek log2(e) / sqrt(128) + ev, and the running maximum m is
-//   taken over x, so P_j = 2^(x_j - m + 14) <= 2^14 carries V's scale and never
-//   overflows f16 (full precision down to 2^-28 of the largest); P V adds up to
-//   the numerator, sum_j P_j 2^-ev (fp32, before P is rounded) to the
-//   denominator, and 2^(14 - m) cancels.
+//   taken over x, so P_j = 2^(x_j - m + 5) carries V's scale; m follows the maximum
+//   only when that has grown by more than 2^8, so P_j <= 2^13 never overflows f16
+//   (full precision down to 2^-19 of the largest, steps of 2^-29 of it below);
+//   P V adds up to the numerator, sum_j P_j 2^-ev (fp32, before P is rounded) to the
+//   denominator, and 2^(5 - m) cancels.
 //
 // Masked keys have x = -inf.  Rows past a sequence's length are whatever the
 // block held before; they, and NaN in a value that only some rows of a tile see,
@@ -37,7 +38,7 @@ struct KvAttnParams {
   float scale_log2;          // log2(e) / sqrt(128)
 };
 
-constexpr float kPBias = 14.f;
+constexpr float kPBias = 5.f, kLag = 8.f;  // P <= 2^(5 + 8)
 
 __device__ __forceinline__ uint32_t f16x2_pack(float lo, float hi) {
   uint32_t d;
@@ -132,7 +133,7 @@ __device__ __forceinline__ uint4 clean_chunk(uint4 u, int key, int length, bool 
 // a cluster of `split` CTAs shares the keys of a row tile, and the partial
 // results meet through distributed shared memory.
 // ---------------------------------------------------------------------------
-constexpr int kFewMaxRows = 64;  // packed rows of a key head; beyond, kvattend_many.cuh
+constexpr int kFewMaxRows = 16;  // packed rows of a key head; beyond, kvattend_many.cuh
 constexpr int kUnitKeys = 32;
 constexpr int kUnitBytes = kUnitKeys * kCacheDim;  // of K, and of V
 constexpr int kFewWarps = 4;
@@ -353,12 +354,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       for (int half = 0; half < 2; ++half) {
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-        const float next = fmaxf(m[half], top[half]);
-        const float safe = next == -INFINITY ? 0.f : next;
-        corr[half] = ex2_approx(m[half] - safe);
-        grown |= next != m[half];
-        m[half] = next;
-        base[half] = kPBias - safe;
+        // A maximum that grows by at most 2^kLag is left as it is: P stays below f16's range.
+        const bool g = top[half] > m[half] + kLag || (m[half] == -INFINITY && top[half] > m[half]);
+        corr[half] = g ? ex2_approx(m[half] - top[half]) : 1.f;
+        grown |= g;
+        if (g) m[half] = top[half];
+        base[half] = kPBias - (m[half] == -INFINITY ? 0.f : m[half]);
       }
       float sum[2] = {0.f, 0.f};
 #pragma unroll

@@ -5,11 +5,13 @@
 // Bound: the tensor cores and the exponentials, about even (512 flops and one
 // exp2 a (row, key); 4096 f16 multiply-adds and 16 exp2 a clock and SM make 128
 // rows x 64 keys 512 clocks of either), with shared memory close behind.  So
-//   - a converted block serves both tiles;
+//   - a converted block serves both tiles; a CTA with at most 128 rows has them in both,
+//     the even steps in one and the odd steps in the other;
 //   - each tile has two S buffers: S of step j + 1 is there before P of step j is,
 //     so neither the warps nor the tensor cores wait for a step's whole chain;
 //   - the rows go from global memory to registers two steps ahead, never through
-//     shared memory in 8 bits.
+//     shared memory in 8 bits (a ring of raw blocks there left room for three operand
+//     stages instead of five: 107 instead of 62 us for 32 rows over 16384, 24 heads).
 //
 //   warps 8-11, 12-15  softmax of tile 0 and 1, a query row a thread: Q to f16 in shared
 //                   memory once; per step the row maximum, P = 2^(x - m) in f16 over
@@ -37,13 +39,16 @@ constexpr int kManySoftmaxWarps = 8, kManyConvWarps = 4;
 // Warps in the order of their urgency: the scheduler prefers older ones.
 constexpr int kManyConvWarp0 = 4, kManySoftmaxWarp0 = 8;
 constexpr int kManyThreads = 16 * 32;
+// Registers a thread, by warpgroup: the launch gives every thread 128 (65536 / 512); the warpgroup of the issuing
+// threads hands over what the others take (64 + 144 + 2 * 152 = 4 * 128).
+constexpr int kManyLaunchRegs = 128, kManyMmaRegs = 64, kManyConvRegs = 144, kManySoftmaxRegs = 152;
+static_assert(kManyMmaRegs + kManyConvRegs + 2 * kManySoftmaxRegs <= 4 * kManyLaunchRegs, "register split");
 constexpr int kManyHalf = kManyStep * 64 * 2;   // 64 rows x 64 f16: half of an operand tile
 constexpr int kManyOperand = 2 * kManyHalf;     // 16 KB
 constexpr int kManyStages = 5;                  // of K, and of V
 constexpr int kManyQuery = 2 * 128 * 64 * 2;    // Q of a tile: two halves of 128 rows x 64 f16
 constexpr int kManyData = 2 * kManyQuery + 2 * kManyStages * kManyOperand;
 constexpr int kManyPitch = kCacheDim + 4;       // floats between rows of a partial result
-constexpr float kManyBias = 5.f, kManyLag = 8.f;  // P <= 2^(5 + 8)
 constexpr uint32_t kManyO = 256;  // TMEM column of tile 0's O
 
 // f16 operands (K-major A; B K-major or, with bit 16, MN-major), fp32 accumulator.
@@ -60,6 +65,14 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+template <int kRegs>
+__device__ __forceinline__ void set_registers() {
+  if constexpr (kRegs < kManyLaunchRegs)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 // (a.x * f + c, a.y * f + c) in one instruction.
@@ -97,7 +110,7 @@ struct ManyShared {
 constexpr int kManySmem = 1024 + kManyData + int(sizeof(ManyShared));
 static_assert(kManySmem <= 232448, "227 KB a CTA");
 static_assert(kManyRows * (kManyPitch * 4 + 8) <= kManyData, "partial rows fit the operands' place");
-static_assert(kManyStages + 2 < 8, "a step's scales outlive its K stage");
+static_assert(kManyStages + 2 < 8, "a step's scales outlive its stage");
 
 __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const KvAttnParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -113,7 +126,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   const int tile = int(gridDim.x / split) - 1 - int(blockIdx.x) / split, rank = int(blockIdx.x) % split;
   const int total_rows = p.nq * p.group, row0 = tile * kManyRows;
   const int rows = min(kManyRows, total_rows - row0);
-  const int tiles = rows > 128 ? 2 : 1;
+  const bool dual = rows <= 128;  // both tiles hold the same rows and take every second step
+  const int stride = dual ? 2 : 1;
 
   if (threadIdx.x == 0) {
     mbar_init(smem_addr(&sh.q_full), kManySoftmaxWarps);
@@ -126,7 +140,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       }
       for (int s = 0; s < kManyStages; ++s) {
         mbar_init(smem_addr(&sh.full[x][s]), kManyConvWarps);
-        mbar_init(smem_addr(&sh.empty[x][s]), uint32_t(tiles));
+        mbar_init(smem_addr(&sh.empty[x][s]), dual ? 1 : 2);  // tiles that read a step
       }
     }
     sh.abort_flag = 0;
@@ -155,9 +169,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
 
   if (warp < kManyConvWarp0) {
     // ------------------------------------------------------------ products
+    set_registers<kManyMmaRegs>();
     // The elected lane runs the whole loop: its operands then stay in uniform registers (11 cycles to issue a
     // product; 27 with a lane elected for each group of products, 54 from a lane chosen by its index).
-    if (warp < tiles && steps > 0 && elect_one()) {
+    if (warp < 2 && (dual ? warp : 0) < steps && elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_f16(128, kManyStep);
       constexpr uint32_t idesc_o = umma_idesc_f16(128, kCacheDim) | (1u << 16);  // V MN-major
       const int x = warp;
@@ -175,43 +190,46 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         umma_commit(smem_addr(&sh.s_full[x][i]));
         umma_commit(smem_addr(&sh.empty[0][s]));
       };
-      bool ok = wait(&sh.q_full, 0u) && wait(&sh.full[0][0], 0u);
+      const int first_step = dual ? x : 0;
+      bool ok = wait(&sh.q_full, 0u) && wait(&sh.full[0][first_step], 0u);
       tc_fence_after();
-      if (ok) issue_s(0, 0);
-      int s = 0, n = 1;            // stages of steps j and j + 1
-      uint32_t ph = 0, phn = 0;    // and their phases
-      for (int j = 0; j < steps && ok; ++j) {
-        // S of step j + 1 goes over P of step j - 1: that step's product must be complete (products of different
-        // shapes are not ordered among themselves).
-        if (j + 1 < steps) {
-          ok = wait(&sh.full[0][n], phn) && (j == 0 || wait(&sh.o_step[x], uint32_t(j - 1) & 1u));
+      if (ok) issue_s(0, first_step);
+      int s = first_step, n = (first_step + stride) % kManyStages;  // stages of this tile's steps i and i + 1
+      uint32_t ph = 0, phn = first_step + stride >= kManyStages;    // and their phases
+      for (int i = 0, j = first_step; j < steps && ok; ++i, j += stride) {
+        // S of the next step goes over P of the one before: that step's product must be complete (products of
+        // different shapes are not ordered among themselves).
+        if (j + stride < steps) {
+          ok = wait(&sh.full[0][n], phn) && (i == 0 || wait(&sh.o_step[x], uint32_t(i - 1) & 1u));
           if (!ok) break;
           tc_fence_after();
-          issue_s((j + 1) & 1, n);
+          issue_s((i + 1) & 1, n);
         }
-        ok = wait(&sh.full[1][s], ph) && wait(&sh.p_full[x][j & 1], uint32_t(j >> 1) & 1u);
+        ok = wait(&sh.full[1][s], ph) && wait(&sh.p_full[x][i & 1], uint32_t(i >> 1) & 1u);
         if (!ok) break;
         tc_fence_after();
         const uint32_t va = smem_addr(operand(1, s));
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_f16_ts(to, ts + (j & 1) * 64 + k * 8,
+          umma_f16_ts(to, ts + (i & 1) * 64 + k * 8,
                       umma_desc_sw128_mn(va + uint32_t(k) * 2 * kVGroupBytes, kManyHalf, kVGroupBytes), idesc_o,
-                      (j | k) ? 1u : 0u);
+                      (i | k) ? 1u : 0u);
         umma_commit(smem_addr(&sh.o_step[x]));
         umma_commit(smem_addr(&sh.empty[1][s]));
         s = n, ph = phn;
-        if (++n == kManyStages) n = 0, phn ^= 1u;
+        n += stride;
+        if (n >= kManyStages) n -= kManyStages, phn ^= 1u;
       }
       umma_commit(smem_addr(&sh.o_last[x]));
     }
     __syncwarp();
-    if (split > 1) {  // the softmax warps' two cluster barriers
+    if (split > 1 || dual) {  // the softmax warps' two cluster barriers
       cluster_sync();
       cluster_sync();
     }
   } else if (warp < kManySoftmaxWarp0) {
     // ------------------------------------------------------------ e4m3 -> f16
+    set_registers<kManyConvRegs>();
     // Thread: 16 bytes `chunk` (dims 16 chunk ..) of rows r0 + 16 i of the block.  Eight neighbouring lanes store
     // four chunks of an even and of an odd row: eight different 16-byte columns of the swizzle.
     const int tid = threadIdx.x - kManyConvWarp0 * 32;
@@ -306,17 +324,19 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       }
     }
     __syncwarp();
-    if (split > 1) {
+    if (split > 1 || dual) {
       cluster_sync();
       cluster_sync();
     }
   } else {
     // ------------------------------------------------------------ softmax
+    set_registers<kManySoftmaxRegs>();
     const int r = threadIdx.x - kManySoftmaxWarp0 * 32, x = (warp - kManySoftmaxWarp0) >> 2;  // row of 256; tile
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t to = tmem + kManyO + x * 128 + lanes;
-    const bool live = r < rows;
-    const int row = row0 + (live ? r : 0), token = row / p.group, head = kh * p.group + row - token * p.group;
+    const int rr = dual ? r & 127 : r;
+    const bool live = rr < rows;
+    const int row = row0 + (live ? rr : 0), token = row / p.group, head = kh * p.group + row - token * p.group;
     const int seen = live ? keys_seen(length, p.nq, token, p.causal) : 0;
     bool ok = true;
     float qf;
@@ -347,11 +367,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       if (lane == 0) mbar_arrive_local(smem_addr(&sh.q_full));
     }
     float m = -INFINITY, l = 0.f;
-    if (x < tiles) {
-      for (int j = 0; j < steps; ++j) {
-        const uint32_t ts = tmem + x * 128 + (j & 1) * 64 + lanes;
+    const int mine = dual ? (steps - x + 1) / 2 : steps;  // steps of this tile
+    {
+      for (int i = 0; i < mine; ++i) {
+        const int j = dual ? 2 * i + x : i;
+        const uint32_t ts = tmem + x * 128 + (i & 1) * 64 + lanes;
         if (lane == 0)
-          ok = wait_spin(smem_addr(&sh.s_full[x][j & 1]), uint32_t(j >> 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
+          ok = wait_spin(smem_addr(&sh.s_full[x][i & 1]), uint32_t(i >> 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
         ok = __shfl_sync(0xffffffffu, int(ok), 0);
         if (!ok) break;
         tc_fence_after();
@@ -379,15 +401,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         const float u = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), f = qf * sc.kf;
         // A block that is not there has ev -inf; nothing seen leaves u at -inf.
         const float top = u == -INFINITY ? -INFINITY : fmaf(u, f, sc.ev);
-        // A maximum that grows by at most 2^kManyLag is left as it is.
-        const bool grown = top > m + kManyLag || (m == -INFINITY && top > m);
+        // A maximum that grows by at most 2^kLag is left as it is.
+        const bool grown = top > m + kLag || (m == -INFINITY && top > m);
         float corr = 1.f;
         if (grown) {
           corr = ex2_approx(m - top);
           m = top;
           l *= corr;
         }
-        const float base = sc.ev - (m == -INFINITY ? 0.f : m) + kManyBias;
+        const float base = sc.ev - (m == -INFINITY ? 0.f : m) + kPBias;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t out[32];
 #pragma unroll
@@ -401,9 +423,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         }
         tmem_st32(ts, out);
         l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), sc.back, l);
-        if (__any_sync(0xffffffffu, grown) && j > 0) {
+        if (__any_sync(0xffffffffu, grown) && i > 0) {
           if (lane == 0)
-            ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(j - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
+            ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(i - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
           ok = __shfl_sync(0xffffffffu, int(ok), 0);
           if (!ok) break;
           tc_fence_after();
@@ -420,20 +442,21 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_local(smem_addr(&sh.p_full[x][j & 1]));
+        if (lane == 0) mbar_arrive_local(smem_addr(&sh.p_full[x][i & 1]));
       }
     }
-    if (steps > 0 && ok) {
+    if (ok) {
       // Both tiles: the operands' place is reused below.
       if (lane == 0)
-        for (int y = 0; y < tiles; ++y)
-          ok = ok && wait_spin(smem_addr(&sh.o_last[y]), 0u, abort, c.status, WAMFFN_DEV_TIMEOUT);
+        for (int y = 0; y < 2; ++y)
+          if ((dual ? y : 0) < steps)
+            ok = ok && wait_spin(smem_addr(&sh.o_last[y]), 0u, abort, c.status, WAMFFN_DEV_TIMEOUT);
       ok = __shfl_sync(0xffffffffu, int(ok), 0);
       tc_fence_after();
     }
     // 32 dims of this row's O; a NaN that was cleaned out of a value this row sees comes back.
     auto load_o = [&](int q, uint32_t (&v)[32]) {
-      if (steps > 0) {
+      if (mine > 0) {
         tmem_ld32(to + q * 32, v);
         tmem_wait_ld(v);
       } else {
@@ -445,10 +468,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         for (int i = 0; i < 32; ++i)
           if (sh.nan_key[q * 32 + i] < seen) v[i] = 0x7fffffffu;
     };
-    if (split == 1) {
+    if (split == 1 && !dual) {
       const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
       __nv_bfloat16* dst = p.out + ((size_t(b) * p.nq + token) * p.heads + head) * kCacheDim;
-      if (x < tiles && ok) {
+      if (ok) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           uint32_t v[32];
@@ -468,16 +491,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       // This CTA's partial rows (unnormalised O, maximum, normaliser) to shared memory; every product has read it.
       float* part = reinterpret_cast<float*>(smem);
       float2* part_ml = reinterpret_cast<float2*>(part + kManyRows * kManyPitch);
-      if (x < tiles) {
+      if (live) {
         part_ml[r] = make_float2(m, l);
+      }
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t v[32];
-          load_o(q, v);
+      for (int q = 0; q < 4; ++q) {
+        uint32_t v[32];
+        load_o(q, v);
+        if (live)
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<uint4*>(part + r * kManyPitch + q * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        }
       }
       __syncwarp();
       cluster_sync();
@@ -485,12 +509,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       const int pieces = ((rows - rank + split - 1) / split) * (kCacheDim / 4);
       for (int i = r; i < pieces; i += kManySoftmaxWarps * 32) {
         const int pr = rank + (i >> 5) * split, d = (i & 31) * 4;
-        const uint32_t ml_at = smem_addr(&part_ml[pr]), o_at = smem_addr(part + pr * kManyPitch + d);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float top = -INFINITY, sum = 0.f;
-        for (int k = 0; k < split; ++k) {
-          const float2 ml = ld_cluster2(map_to_cta(ml_at, k));
-          const float4 u = ld_cluster4(map_to_cta(o_at, k));
+        for (int k = 0; k < split * stride; ++k) {  // CTA, and tile where both hold the row
+          const int from = dual ? k >> 1 : k, at = pr + (dual ? 128 * (k & 1) : 0);
+          const float2 ml = ld_cluster2(map_to_cta(smem_addr(&part_ml[at]), from));
+          const float4 u = ld_cluster4(map_to_cta(smem_addr(part + at * kManyPitch + d), from));
           const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
           const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
           v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
