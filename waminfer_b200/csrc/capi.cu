@@ -167,9 +167,7 @@ int prepare_device(int device, int* sm_count) {
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(masked_attention_kernel<true, true>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem));
-    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
-    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
-    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
     // The kernel's warpgroups trade registers: a split that the launch does not bring would wait for good.
     cudaFuncAttributes many_attr{};
@@ -2035,7 +2033,7 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   if (rows > 0x7fffffff / 16) return fail(WAMFFN_ERR_INVALID, "too many query rows");
   int sm = 0;
   if ((rc = prepare_current_device(&sm))) return rc;
-  if (rows > kFewMaxRows) {
+  if (rows > kFewRows) {
     const int64_t row_tiles = (rows + kManyRows - 1) / kManyRows, ctas = row_tiles * p.c.kv_heads * p.c.batch;
     // Key split: the one with the least waves x (steps of a CTA + what a CTA costs besides, about four steps);
     // clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
@@ -2054,23 +2052,19 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
     return launch_pdl(kv_attend_many_kernel, dim3(unsigned(row_tiles * p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
                       kManyThreads, kManySmem, p.split, stream, p);
   }
-  const int tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t row_tiles = (rows + 16 * tiles - 1) / (16 * tiles);
-  // Key split: enough CTAs for two an SM, as long as a key group has a unit; and beyond that as long as it has
+  // Key split: enough CTAs for three an SM, as long as a warp has a unit; and beyond that as long as it has
   // sixteen, so that ragged sequences even out over several waves.
-  const int64_t ctas = row_tiles * p.c.kv_heads * p.c.batch;
-  const int64_t units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys), groups = kFewWarps / tiles;
+  const int64_t ctas = int64_t(p.c.kv_heads) * p.c.batch, units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys);
   p.split = 1;
   if (a->key_split)
     p.split = a->key_split;
   else
     for (int s : {2, 4, 8})
-      if (s * groups * 16 <= units || (ctas * s <= 2 * sm && s * groups <= units)) p.split = s;
+      if (s * kFewWarps * 16 <= units || (ctas * s <= 3 * sm && s * kFewWarps <= units)) p.split = s;
   CUtensorMap kmap, vmap;
   if ((rc = encode_cache(&kmap, p.c.keys, p.c, kUnitKeys))) return rc;
   if ((rc = encode_cache(&vmap, p.c.values, p.c, kUnitKeys))) return rc;
-  auto kernel = tiles == 1 ? kv_attend_few_kernel<1> : tiles == 2 ? kv_attend_few_kernel<2> : kv_attend_few_kernel<4>;
-  return launch_pdl(kernel, dim3(unsigned(row_tiles * p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
+  return launch_pdl(kv_attend_few_kernel, dim3(unsigned(p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
                     kFewWarps * 32, kFewSmem, p.split, stream, kmap, vmap, p);
 }
 

@@ -121,55 +121,48 @@ __device__ __forceinline__ uint4 clean_chunk(uint4 u, int key, int length, bool 
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (a decode step, the action rows): warps of 16 packed rows (query
-// token x head of the group), matrix products by mma.sync from registers.
+// Few rows (a decode step: at most 16 packed rows, query token x head of the
+// group): matrix products by mma.sync from registers.
 //
 // Bound: HBM (the cache is read once, 256 bytes a key and head).  A unit is 32
 // keys of one head, 4 KB of K and of V, loaded by TMA with the 128-byte swizzle
 // into a ring; the fragments are converted in registers (a lane takes 16
 // neighbouring dims of K, which the product's order of k allows, and the same
 // 16 dims of four rows of V), so nothing is written back to shared memory.
-// 4 warps: kTiles row tiles x (4 / kTiles) key groups with rings of their own;
-// a cluster of `split` CTAs shares the keys of a row tile, and the partial
-// results meet through distributed shared memory.
+// Four warps with rings and units of their own, three CTAs an SM (168 registers:
+// a unit is one long chain of dependent steps, and warps hide each other's);
+// a cluster of `split` CTAs shares the keys, and the partial results meet through
+// distributed shared memory.
 // ---------------------------------------------------------------------------
-constexpr int kFewMaxRows = 16;  // packed rows of a key head; beyond, kvattend_many.cuh
+constexpr int kFewRows = 16;  // packed rows of a key head at most; beyond, kvattend_many.cuh
 constexpr int kUnitKeys = 32;
 constexpr int kUnitBytes = kUnitKeys * kCacheDim;  // of K, and of V
 constexpr int kFewWarps = 4;
-constexpr int kFewStages = 12;                     // all rings together
+constexpr int kFewStages = 2;                      // of a warp's ring
 constexpr int kFewPitch = kCacheDim + 4;           // floats between rows of a partial result
-constexpr int kFewRing = kFewStages * 2 * kUnitBytes;
-constexpr int kFewSmem = kFewRing + 1024;
+constexpr int kFewRing = kFewStages * 2 * kUnitBytes;  // of a warp
+constexpr int kFewSmem = kFewWarps * kFewRing + 1024;
+static_assert(kFewRows * kFewPitch * 4 <= kFewRing, "a partial result fits its warp's ring");
 
-template <int kTiles>
-__global__ void __launch_bounds__(kFewWarps * 32, 2)
+__global__ void __launch_bounds__(kFewWarps * 32, 3)
     kv_attend_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                          const KvAttnParams p) {
-  constexpr int kGroups = kFewWarps / kTiles;       // key groups
-  constexpr int kStages = kFewStages / kGroups;     // of a group's ring
-  constexpr int kRows = 16 * kTiles;
-  static_assert(kRows * kFewPitch * 4 <= kStages * 2 * kUnitBytes, "a partial result fits its group's ring");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full[kFewStages], empty[kFewStages];
-  __shared__ __align__(16) float2 part_ml[kGroups][kRows];  // (maximum, normaliser) of a group's rows
-  __shared__ __align__(16) float2 cta_ml[kRows];
+  __shared__ __align__(8) uint64_t full[kFewWarps][kFewStages];
+  __shared__ __align__(16) float2 part_ml[kFewWarps][kFewRows];  // (maximum, normaliser) of a warp's rows
+  __shared__ __align__(16) float2 cta_ml[kFewRows];
   __shared__ int nan_key[kCacheDim];
   __shared__ int nan_any;
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kg = warp / kTiles, mt = warp % kTiles;
   const int g = lane >> 2, t = lane & 3;
-  const int split = p.split, tile = int(blockIdx.x) / split, rank = int(blockIdx.x) - tile * split;
+  const int split = p.split, rank = blockIdx.x;
   const int kh = blockIdx.y, b = blockIdx.z;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kFewStages; ++s) {
-      mbar_init(smem_addr(&full[s]), 1);
-      mbar_init(smem_addr(&empty[s]), kTiles);
-    }
+    for (int s = 0; s < kFewWarps * kFewStages; ++s) mbar_init(smem_addr(&full[0][s]), 1);
     nan_any = 0;
     abort_flag = 0;
     fence_mbar_init();
@@ -182,11 +175,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   pdl_launch_dependents();
 
   const CacheView& c = p.c;
-  const int worker = rank * kGroups + kg, workers = split * kGroups;
-  uint8_t* my_ring = ring + kg * kStages * 2 * kUnitBytes;
-  uint64_t* my_full = full + kg * kStages;
-  uint64_t* my_empty = empty + kg * kStages;
-  // Block ids and scales of 32 of this group's units (worker + i * workers) at a time, one a lane.  The scales are
+  const int worker = rank * kFewWarps + warp, workers = split * kFewWarps;
+  uint8_t* my_ring = ring + warp * kFewRing;
+  uint64_t* my_full = full[warp];
+  // Block ids and scales of 32 of this warp's units (worker + i * workers) at a time, one a lane.  The scales are
   // taken apart where they are used: no load waits for them.
   struct Info {
     int id;         // tile row of the unit in the pool's tensor map; -1: bad block id
@@ -208,25 +200,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   };
   const int first_id = table_at(lane);  // on its way together with the length
   const int length = cache_length(c, b);
-  const int total_rows = p.nq * p.group, row0 = tile * kRows;
-  const int rows = min(kRows, total_rows - row0);
-  const int least = keys_seen(length, p.nq, row0 / p.group, p.causal);
-  const int most = keys_seen(length, p.nq, (row0 + rows - 1) / p.group, p.causal);
+  const int rows = p.nq * p.group;
+  const int least = keys_seen(length, p.nq, 0, p.causal), most = keys_seen(length, p.nq, p.nq - 1, p.causal);
   const int units = (most + kUnitKeys - 1) / kUnitKeys;
   const int mine = units > worker ? (units - worker + workers - 1) / workers : 0;
 
-  const bool producer = mt == 0;  // this warp's lane 0 loads for the group
   const uint64_t policy = l2_policy_evict_first();
-  Info ahead = info_of(lane, first_id);  // of the producer's chunk of 32 units
+  Info ahead = info_of(lane, first_id);  // of the units being loaded
   int ahead_chunk = 0, issued = 0;
-  auto issue = [&](int i) {  // whole warp: unit i into stage i % kStages
+  auto issue = [&](int i) {  // unit i into stage i % kFewStages
     if ((i >> 5) != ahead_chunk) {
       ahead_chunk = i >> 5;
       ahead = info_of(ahead_chunk * 32 + lane, table_at(ahead_chunk * 32 + lane));
     }
     const int id = __shfl_sync(0xffffffffu, ahead.id, i & 31);
     if (lane == 0) {
-      const int s = i % kStages;
+      const int s = i % kFewStages;
       const uint32_t bar = smem_addr(&my_full[s]), dst = smem_addr(my_ring + s * 2 * kUnitBytes);
       if (id >= 0) {
         mbar_arrive_expect_tx(bar, 2 * kUnitBytes);
@@ -239,8 +228,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     }
     issued = i + 1;
   };
-  if (producer)
-    for (int i = 0; i < min(mine, kStages); ++i) issue(i);
+  for (int i = 0; i < min(mine, kFewStages); ++i) issue(i);
 
   // Query fragments: rows g and g + 8 of the warp's tile, dims [32 t, 32 t + 32):
   // step ks = 4 c + w takes dims 32 t + 16 c + 4 w + {0, 1} and {2, 3} as its k
@@ -250,8 +238,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   int seen[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int r = row0 + mt * 16 + g + 8 * half;
-    const bool live = r < total_rows;
+    const int r = g + 8 * half;
+    const bool live = r < rows;
     const int token = live ? r / p.group : 0;
     const int head = kh * p.group + (live ? r - token * p.group : 0);
     seen[half] = live ? keys_seen(length, p.nq, token, p.causal) : 0;
@@ -285,15 +273,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   int now_chunk = 0;
   bool ok = true;
   for (int i = 0; i < mine; ++i) {
-    const int s = i % kStages;
-    if (producer && i > 0 && i - 1 + kStages < mine) {  // refill the stage of the previous unit
-      if (kTiles > 1)
-        ok = wait_bounded(smem_addr(&my_empty[(i - 1) % kStages]), uint32_t((i - 1) / kStages) & 1u, &abort_flag,
-                          c.status, WAMFFN_DEV_TIMEOUT);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      issue(i - 1 + kStages);
-    }
+    const int s = i % kFewStages;
     if ((i >> 5) != now_chunk) {
       now_chunk = i >> 5;
       now = info_of(now_chunk * 32 + lane, table_at(now_chunk * 32 + lane));
@@ -301,7 +281,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     const int id = __shfl_sync(0xffffffffu, now.id, i & 31);
     const float kf = exp2_int(scale_exp(__shfl_sync(0xffffffffu, now.ks, i & 31)));
     const int ev = scale_exp(__shfl_sync(0xffffffffu, now.vs, i & 31));
-    ok = wait_bounded(smem_addr(&my_full[s]), uint32_t(i / kStages) & 1u, &abort_flag, c.status, WAMFFN_DEV_TIMEOUT);
+    ok = wait_bounded(smem_addr(&my_full[s]), uint32_t(i / kFewStages) & 1u, &abort_flag, c.status, WAMFFN_DEV_TIMEOUT);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     if (id >= 0) {
@@ -323,10 +303,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
           for (int nt = 0; nt < 4; ++nt)
             mma_f16(x[nt], qa[cc * 4 + e], e4m3x2_to_f16x2(w[nt][e]), e4m3x2_hi_to_f16x2(w[nt][e]));
       }
-      const bool whole = key0 + kUnitKeys <= least;  // every row of the tile sees every key of the unit
+      const bool whole = key0 + kUnitKeys <= least;  // every row sees every key of the unit
       if (!whole) {
-        // Each warp that reads the unit cleans all of it: the warps of a group write the same values.  Rows that
-        // every row of the tile sees need no look.
+        // Keys that every row sees need no look.
 #pragma unroll 1
         for (int e = max(0, (least < most ? least : length) - key0) * 8 + lane; e < kUnitKeys * 8; e += 32) {
           const int row = e >> 3, chunk = e & 7;
@@ -403,20 +382,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         }
       }
     }
-    __syncwarp();
-    if (kTiles > 1 && lane == 0) mbar_arrive_local(smem_addr(&my_empty[s]));
+    __syncwarp();  // the stage has been read
+    if (i + kFewStages < mine) issue(i + kFewStages);
   }
-  if (!ok && producer && lane == 0)  // copies in flight land before the shared memory is given up
-    for (int i = max(0, issued - kStages); i < issued; ++i)
-      wait_drain(smem_addr(&my_full[i % kStages]), uint32_t(i / kStages) & 1u);
+  if (!ok && lane == 0)  // copies in flight land before the shared memory is given up
+    for (int i = max(0, issued - kFewStages); i < issued; ++i)
+      wait_drain(smem_addr(&my_full[i % kFewStages]), uint32_t(i / kFewStages) & 1u);
   __syncthreads();  // every ring is idle: partial results go over them
   float* part = reinterpret_cast<float*>(my_ring);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
     l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-    const int r = mt * 16 + g + 8 * half;
-    if (t == 0) part_ml[kg][r] = make_float2(m[half], l[half]);
+    const int r = g + 8 * half;
+    if (t == 0) part_ml[warp][r] = make_float2(m[half], l[half]);
 #pragma unroll
     for (int n = 0; n < 16; n += 4)
 #pragma unroll
@@ -435,20 +414,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       }
   }
   __syncthreads();
-  // The groups' partial results into group 0's place.
+  // The warps' partial results into warp 0's place.
   for (int i = threadIdx.x; i < rows * (kCacheDim / 4); i += kFewWarps * 32) {
     const int r = i >> 5, d = (i & 31) * 4;
     float top = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) top = fmaxf(top, part_ml[k][r].x);
+    for (int k = 0; k < kFewWarps; ++k) top = fmaxf(top, part_ml[k][r].x);
     const float safe = top == -INFINITY ? 0.f : top;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
+    for (int k = 0; k < kFewWarps; ++k) {
       const float f = ex2_approx(part_ml[k][r].x - safe);
       const float4 u = *reinterpret_cast<const float4*>(
-          reinterpret_cast<const float*>(ring + k * kStages * 2 * kUnitBytes) + r * kFewPitch + d);
+          reinterpret_cast<const float*>(ring + k * kFewRing) + r * kFewPitch + d);
       v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
       sum += part_ml[k][r].y * f;
     }
@@ -488,7 +467,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       sum += ml[k].y * f;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // nothing seen: zeros
-    const int row = row0 + r, token = row / p.group, head = kh * p.group + row - token * p.group;
+    const int token = r / p.group, head = kh * p.group + r - token * p.group;
     if (!abort_flag)
       *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.nq + token) * p.heads + head) * kCacheDim + d) =
           make_uint2(bf2_pack(v.x * inv, v.y * inv), bf2_pack(v.z * inv, v.w * inv));
