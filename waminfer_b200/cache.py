@@ -29,24 +29,24 @@ HEAD_DIM = 128
 FORMAT = torch.float8_e4m3fn
 
 
-def _rows(t: torch.Tensor, name: str, batch: int, width: int, device: torch.device) -> torch.Tensor:
-    """A [batch, rows, width] bf16 operand that the kernels can read in place, else a copy."""
+def _rows(t: torch.Tensor, name: str, batch: int, width: int,
+          device: torch.device) -> tuple[_lib.RowsView, torch.Tensor]:
+    """View of a [batch, rows, width] bf16 operand, and the tensor it views (a
+    copy if the kernels cannot read its rows in place)."""
     if t.dim() != 3 or t.dtype != torch.bfloat16 or t.device != device:
         raise ValueError(f"{name} must be a bf16 tensor [batch, rows, heads * {HEAD_DIM}] on {device}")
-    if t.shape[0] != batch or t.shape[2] != width:
+    count, rows, held = t.shape
+    if count != batch or held != width:
         raise ValueError(f"{name} {tuple(t.shape)}: expected [{batch}, rows, {width}]")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the 8-bit cache has no backward pass: run it with gradients disabled")
     sb, sr, se = t.stride()
-    if se != 1 or sb % 8 or sr % 8 or t.data_ptr() % 16 or (sr < width and t.shape[1] > 1):
+    if se != 1 or sb % 8 or sr % 8 or t.data_ptr() % 16 or (sr < width and rows > 1):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
-
-
-def _view(t: torch.Tensor) -> _lib.RowsView:
-    return _lib.RowsView(t.data_ptr(), t.stride(1), t.stride(0))
+        sb, sr, _ = t.stride()
+    return _lib.RowsView(t.data_ptr(), sr, sb), t
 
 
 def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
@@ -147,12 +147,13 @@ class KVCache8:
         beyond its length, a block id outside the pool) keeps what it had, and
         ``status`` reports it."""
         width = self.kv_heads * HEAD_DIM
-        k, v = _rows(k, "k", self.batch, width, self.device), _rows(v, "v", self.batch, width, self.device)
+        (k_view, k), (v_view, v) = (_rows(k, "k", self.batch, width, self.device),
+                                    _rows(v, "v", self.batch, width, self.device))
         if k.shape != v.shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
         if k.shape[1] == 0:
             raise ValueError("append needs at least one row (counts may be zero)")
-        args = _lib.CacheAppendArgs(self._view, _view(k), _view(v), None if counts is None else self._index(
+        args = _lib.CacheAppendArgs(self._view, k_view, v_view, None if counts is None else self._index(
             "counts", counts), None if at is None else self._index("at", at), k.shape[1])
         _lib.launch(_lib.lib().wamffn_cache_append, self.device.index, ctypes.byref(args))
 
@@ -179,11 +180,12 @@ class KVCache8:
         keys (0 = chosen; 1, 2, 4, 8)."""
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"heads={heads} must be a multiple of the cache's {self.kv_heads}")
-        q = _rows(q, "q", self.batch, heads * HEAD_DIM, self.device)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if q.shape[1] == 0:
+        view, q = _rows(q, "q", self.batch, heads * HEAD_DIM, self.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        rows = q.shape[1]
+        if rows == 0:
             return out
-        args = _lib.CacheAttentionArgs(self._view, _view(q), out.data_ptr(), q.shape[1], heads, causal, key_split)
+        args = _lib.CacheAttentionArgs(self._view, view, out.data_ptr(), rows, heads, causal, key_split)
         _lib.launch(_lib.lib().wamffn_cache_attention, self.device.index, ctypes.byref(args))
         return out
 

@@ -1815,7 +1815,6 @@ int prepare_current_device(int* sm_count) {
 template <int D, bool kInter>
 int launch_rope(const RopeParams& p, bool whole_row, int sm, void* stream) {
   const int heads = p.q.heads + p.k.heads;
-  const int64_t tokens = int64_t(p.batch) * p.rows;
   if (whole_row) {
     const int vec = heads * (D / 8);
     const int per = vec <= 512 ? 1 : vec <= 1024 ? 2 : vec <= 2048 ? 4 : 8;
@@ -1824,15 +1823,19 @@ int launch_rope(const RopeParams& p, bool whole_row, int sm, void* stream) {
                   : per == 2 ? rope_row_kernel<D, kInter, 2>
                   : per == 4 ? rope_row_kernel<D, kInter, 4>
                              : rope_row_kernel<D, kInter, 8>;
-    return launch_pdl(kernel, dim3(unsigned(tokens)), threads, 0, 1, stream, p);
+    return launch_pdl(kernel, dim3(unsigned(p.rows), unsigned(p.batch)), threads, 0, 1, stream, p);
   }
   constexpr int groups = kRopeThreads / (D / 8);
-  auto ctas = [&](int per) { return (tokens * ((heads + per - 1) / per) + groups - 1) / groups; };
-  if (ctas(4) > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many rows");
-  // Four heads a group read the table once for the four and keep four loads a
-  // lane in flight; while that leaves SMs idle, one head a group.
-  if (ctas(4) >= 2 * sm) return launch_pdl(rope_head_kernel<D, kInter, 4>, dim3(unsigned(ctas(4))), kRopeThreads, 0, 1, stream, p);
-  return launch_pdl(rope_head_kernel<D, kInter, 1>, dim3(unsigned(ctas(1))), kRopeThreads, 0, 1, stream, p);
+  auto ctas = [&](int per) {
+    const int chunks = (p.q.heads + per - 1) / per + (p.k.heads + per - 1) / per;
+    return (int64_t(p.rows) * chunks + groups - 1) / groups;
+  };
+  if (ctas(1) > 0x7fffffff / groups) return fail(WAMFFN_ERR_INVALID, "too many rows");
+  // Eight heads a group read the table and make its factors once for the eight
+  // and keep eight loads a lane in flight; while that leaves SMs idle, one head a group.
+  const bool many = ctas(8) * p.batch >= 2 * sm;
+  auto kernel = many ? rope_head_kernel<D, kInter, 8> : rope_head_kernel<D, kInter, 1>;
+  return launch_pdl(kernel, dim3(unsigned(ctas(many ? 8 : 1)), unsigned(p.batch)), kRopeThreads, 0, 1, stream, p);
 }
 
 // Clusters of `split` CTAs of kv_attend_many_kernel that the current device holds at once.
@@ -1912,7 +1915,7 @@ int wamffn_qk_norm_rope(void* stream, const wamffn_qk_rope_args* a) {
     return fail(WAMFFN_ERR_UNSUPPORTED, "head_dim=%d: 64, 128 or 256", d);
   if (a->batch < 1 || a->rows < 1 || a->heads < 1 || a->kv_heads < 0 || a->heads > 65536 || a->kv_heads > 65536)
     return fail(WAMFFN_ERR_INVALID, "batch=%d rows=%d heads=%d kv_heads=%d", a->batch, a->rows, a->heads, a->kv_heads);
-  if (int64_t(a->batch) * a->rows > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many rows");
+  if (a->batch > 65535) return fail(WAMFFN_ERR_UNSUPPORTED, "batch=%d: up to 65535", a->batch);
   int rc = check_rows_view(a->q, int64_t(a->heads) * d, a->rows, a->batch, "q");
   if (rc) return rc;
   if (a->kv_heads && (rc = check_rows_view(a->k, int64_t(a->kv_heads) * d, a->rows, a->batch, "k"))) return rc;
@@ -1983,8 +1986,9 @@ int wamffn_cache_append(void* stream, const wamffn_cache_append_args* a) {
   p.at = a->at;
   p.rows = a->rows;
   p.places = int(std::min<int64_t>((int64_t(a->rows) + 2 * kCacheBlock - 2) / kCacheBlock, p.c.width));
-  return launch_pdl(cache_append_kernel, dim3(unsigned(p.places), unsigned(2 * p.c.kv_heads), unsigned(p.c.batch)),
-                    kAppendThreads, 0, 1, stream, p);
+  const int64_t ctas = int64_t(p.places) * 2 * p.c.kv_heads;
+  if (ctas > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many rows");
+  return launch_pdl(cache_append_kernel, dim3(unsigned(ctas), unsigned(p.c.batch)), kAppendThreads, 0, 1, stream, p);
 }
 
 int wamffn_cache_read(void* stream, const wamffn_cache_read_args* a) {
@@ -2002,10 +2006,9 @@ int wamffn_cache_read(void* stream, const wamffn_cache_read_args* a) {
   p.count = a->count;
   p.k = static_cast<__nv_bfloat16*>(a->k);
   p.v = static_cast<__nv_bfloat16*>(a->v);
-  return launch_pdl(cache_read_kernel,
-                    dim3(unsigned((int64_t(a->count) + kReadRows - 1) / kReadRows), unsigned(2 * p.c.kv_heads),
-                         unsigned(p.c.batch)),
-                    kReadThreads, 0, 1, stream, p);
+  const int64_t ctas = (int64_t(a->count) + kReadRows - 1) / kReadRows * 2 * p.c.kv_heads;
+  if (ctas > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many rows");
+  return launch_pdl(cache_read_kernel, dim3(unsigned(ctas), unsigned(p.c.batch)), kReadThreads, 0, 1, stream, p);
 }
 
 int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {

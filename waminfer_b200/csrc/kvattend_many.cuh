@@ -369,11 +369,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
     float m = -INFINITY, l = 0.f;
     const int mine = dual ? (steps - x + 1) / 2 : steps;  // steps of this tile
     {
-      for (int i = 0; i < mine; ++i) {
-        const int j = dual ? 2 * i + x : i;
-        const uint32_t ts = tmem + x * 128 + (i & 1) * 64 + lanes;
+      for (int n = 0; n < mine; ++n) {
+        const int j = dual ? 2 * n + x : n;
+        const uint32_t ts = tmem + x * 128 + (n & 1) * 64 + lanes;
         if (lane == 0)
-          ok = wait_spin(smem_addr(&sh.s_full[x][i & 1]), uint32_t(i >> 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
+          ok = wait_spin(smem_addr(&sh.s_full[x][n & 1]), uint32_t(n >> 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
         ok = __shfl_sync(0xffffffffu, int(ok), 0);
         if (!ok) break;
         tc_fence_after();
@@ -423,9 +423,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         }
         tmem_st32(ts, out);
         l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), sc.back, l);
-        if (__any_sync(0xffffffffu, grown) && i > 0) {
+        if (__any_sync(0xffffffffu, grown) && n > 0) {
           if (lane == 0)
-            ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(i - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
+            ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(n - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
           ok = __shfl_sync(0xffffffffu, int(ok), 0);
           if (!ok) break;
           tc_fence_after();
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_local(smem_addr(&sh.p_full[x][i & 1]));
+        if (lane == 0) mbar_arrive_local(smem_addr(&sh.p_full[x][n & 1]));
       }
     }
     if (ok) {

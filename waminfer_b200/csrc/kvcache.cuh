@@ -89,65 +89,69 @@ struct AppendParams {
 
 constexpr int kAppendThreads = 128;
 
-// One CTA a (touched block, head, batch) of the keys or of the values: largest
+// One CTA a (touched block, head, batch) of the keys or of the values (neighbouring
+// CTAs take neighbouring heads of the same rows, which lie side by side in k and v): largest
 // magnitude of its new rows, scale, conversion.  The rows that the block holds
 // already are rewritten only where its scale grows.  A sequence whose rows do not
 // fit (past its table, behind a gap, through a block id outside the pool) is left
-// as it is, and the status word gets WAMFFN_DEV_BAD_INDEX.  The last CTA of a
-// sequence to have read its length writes the new one.
+// as it is, and the status word gets WAMFFN_DEV_BAD_INDEX.
 __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const AppendParams p) {
   __shared__ uint32_t tops[kAppendThreads / 32];
   pdl_wait_prior();
   pdl_launch_dependents();
   const CacheView& c = p.c;
-  const int b = blockIdx.z, h = blockIdx.y >> 1, place = blockIdx.x;
-  const bool value = blockIdx.y & 1;
+  const int b = blockIdx.y, place = blockIdx.x / (2 * c.kv_heads), side = blockIdx.x % (2 * c.kv_heads);
+  const bool value = side >= c.kv_heads;
+  const int h = value ? side - c.kv_heads : side;
   const int tid = threadIdx.x;
   const int length = c.lengths[b];
   const long long at = p.at ? p.at[b] : length;
   const long long count = p.counts ? max(0, min(p.counts[b], p.rows)) : p.rows;
   const long long end = at + count;
+  const long long first = at / kCacheBlock, low = (first + place) * kCacheBlock;  // the block's first row in the sequence
   bool good = at >= 0 && at <= length && end <= (long long)c.width * kCacheBlock;
-  const long long first = at / kCacheBlock;
   const int* table = c.table + b * c.table_stride;
+  const int lo = int(max(at - low, 0ll)), hi = good ? int(max(min(end - low, (long long)kCacheBlock), 0ll)) : 0;  // new rows
+  // The rows are on their way while the block ids are looked over.
+  const __nv_bfloat16* x = value ? p.v + b * p.v_batch + h * kCacheDim : p.k + b * p.k_batch + h * kCacheDim;
+  const long long stride = value ? p.v_row : p.k_row;
+  const int lane = tid & 15;       // 8 dims of a row
+  constexpr int kStep = kAppendThreads / 16, kPer = kCacheBlock / kStep;
+  uint4 u[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int r = lo + (tid >> 4) + i * kStep;
+    u[i] = r < hi ? *reinterpret_cast<const uint4*>(x + (low + r - at) * stride + lane * 8) : make_uint4(0, 0, 0, 0);
+  }
   if (good)
     for (long long i = first + tid; i * kCacheBlock < end; i += kAppendThreads) {
       const int id = table[i];
       good = good && id >= 0 && id < c.blocks;
     }
   good = __syncthreads_and(good);
-  if (tid == 0) {  // every CTA of the sequence has read its length before the last one writes it
+  // The last CTA of a sequence to have read its length writes the new one (in flight while the rows are stored).
+  int ticket = -1;
+  if (tid == 0) {
     if (!good && c.status) atomicOr(c.status, WAMFFN_DEV_BAD_INDEX);
-    const int total = int(gridDim.x * gridDim.y);
-    __threadfence();
-    if (atomicAdd(&c.tickets[b], 1) == total - 1) {
+    ticket = atomicAdd(&c.tickets[b], 1);
+  }
+  auto leave = [&]() {
+    if (ticket == int(gridDim.x) - 1) {
       c.tickets[b] = 0;
       if (good) c.lengths[b] = int(end);
     }
-  }
-  const long long low = (first + place) * kCacheBlock;  // the block's first row in the sequence
-  if (!good || count == 0 || low >= end) return;
+  };
+  if (!good || count == 0 || low >= end) return leave();
   const size_t tile = size_t(table[first + place]) * c.kv_heads + h;
   uint8_t* codes = (value ? c.values : c.keys) + tile * kCacheTile;
   float* scale = (value ? c.value_scales : c.key_scales) + tile;
-  const __nv_bfloat16* x = value ? p.v + b * p.v_batch + h * kCacheDim : p.k + b * p.k_batch + h * kCacheDim;
-  const long long stride = value ? p.v_row : p.k_row;
-  const int lo = int(max(at - low, 0ll)), hi = int(min(end - low, (long long)kCacheBlock));  // new rows of the block
-  const int lane = tid & 15;       // 8 dims of a row
-  constexpr int kStep = kAppendThreads / 16, kPer = kCacheBlock / kStep;
-  uint4 u[kPer];
+  const int held = lo > 0 ? scale_exp(*scale) : kCacheLeastExp;  // the block's scale, while it holds rows
   uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int r = lo + (tid >> 4) + i * kStep;
-    u[i] = r < hi ? *reinterpret_cast<const uint4*>(x + (low + r - at) * stride + lane * 8) : make_uint4(0, 0, 0, 0);
-  }
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
     top = finite_max(finite_max(finite_max(finite_max(top, u[i].x), u[i].y), u[i].z), u[i].w);
   top = __reduce_max_sync(0xffffffffu, top);
   if ((tid & 31) == 0) tops[tid >> 5] = top;
-  const int held = lo > 0 ? scale_exp(*scale) : kCacheLeastExp;  // the block's scale, while it holds rows
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, tops[w]);
@@ -172,6 +176,7 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
     }
   }
   if (tid == 0) *scale = exp2_int(e);
+  leave();
 }
 
 struct CacheReadParams {
@@ -190,9 +195,10 @@ __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const CacheRea
   pdl_wait_prior();
   pdl_launch_dependents();
   const CacheView& c = p.c;
-  const int b = blockIdx.z, h = blockIdx.y >> 1;
-  const bool value = blockIdx.y & 1;
-  const int i = blockIdx.x * kReadRows + (threadIdx.x >> 3), lane = threadIdx.x & 7;
+  const int b = blockIdx.y, side = blockIdx.x % (2 * c.kv_heads);  // as the store: heads side by side
+  const bool value = side >= c.kv_heads;
+  const int h = value ? side - c.kv_heads : side;
+  const int i = int(blockIdx.x / (2 * c.kv_heads)) * kReadRows + (threadIdx.x >> 3), lane = threadIdx.x & 7;
   if (i >= p.count) return;
   const long long row = (long long)(p.start ? p.start[b] : p.start_all) + i;
   uint32_t out[8] = {};

@@ -110,11 +110,10 @@ __device__ __forceinline__ float rope_squares(const uint4& u) {
 
 // x r w, turned, rounded and stored.  `w` as rope_ld laid it out.
 template <bool kInterleaved>
-__device__ __forceinline__ void rope_store(__nv_bfloat16* head, const RopeDims& d, const uint4& u, const uint4& wu,
+__device__ __forceinline__ void rope_store(__nv_bfloat16* head, const RopeDims& d, const uint4& u, const float (&w)[8],
                                            float r, const float (&c)[4], const float (&s)[4]) {
-  float x[8], w[8], y[8];
+  float x[8], y[8];
   rope_unpack(u, x);
-  rope_unpack(wu, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
   // Pairs inside the lane: (0,1)(2,3)(4,5)(6,7) interleaved, (0,4)(1,5)(2,6)(3,7) in halves.
@@ -135,49 +134,44 @@ __device__ __forceinline__ void rope_store(__nv_bfloat16* head, const RopeDims& 
   }
 }
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 
-// Norm of each head.  A group of D / 8 lanes takes kHeads heads of one token,
-// all loaded before the first is used; queries' heads first, then keys'.
+// Norm of each head.  A group of D / 8 lanes takes up to kHeads heads of one
+// token, all queries' or all keys' (one address and one weight for them), all
+// loaded before the first is used.
 template <int D, bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(kRopeThreads) rope_head_kernel(const RopeParams p) {
   constexpr int kLanes = D / 8, kGroups = kRopeThreads / kLanes;
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int heads = p.q.heads + p.k.heads;
-  const int chunks = (heads + kHeads - 1) / kHeads;
-  const long long item = (long long)blockIdx.x * kGroups + threadIdx.x / kLanes;
-  if (item >= (long long)p.batch * p.rows * chunks) return;  // whole groups leave; the shuffles name their group
-  const long long token = item / chunks;
-  const int h0 = int(item - token * chunks) * kHeads;
-  const int b = int(token / p.rows), t = int(token - (long long)b * p.rows);
+  const int q_chunks = (p.q.heads + kHeads - 1) / kHeads, chunks = q_chunks + (p.k.heads + kHeads - 1) / kHeads;
+  const uint32_t item = blockIdx.x * kGroups + threadIdx.x / kLanes;
+  const int b = blockIdx.y, t = item / uint32_t(chunks), chunk = int(item - uint32_t(t) * chunks);
+  if (t >= p.rows) return;  // whole groups leave; the shuffles name their group
+  const bool key = chunk >= q_chunks;
+  const int heads = key ? p.k.heads : p.q.heads, h0 = (key ? chunk - q_chunks : chunk) * kHeads;
+  const int n = min(kHeads, heads - h0);
+  const __nv_bfloat16* src = (key ? p.k.x : p.q.x) + b * (key ? p.k.batch_stride : p.q.batch_stride) +
+                             t * (key ? p.k.row_stride : p.q.row_stride) + h0 * D;
+  __nv_bfloat16* dst = (key ? p.k.y : p.q.y) + (((long long)b * p.rows + t) * heads + h0) * D;
   const RopeDims d = rope_dims<kInterleaved>(threadIdx.x % kLanes, p.pairs);
   const long long at = p.rope ? rope_position(p, b, t) : 0;
   uint4 x[kHeads];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    const bool key = h >= p.q.heads;
-    const __nv_bfloat16* base = key ? p.k.x + b * p.k.batch_stride + t * p.k.row_stride + (h - p.q.heads) * D
-                                    : p.q.x + b * p.q.batch_stride + t * p.q.row_stride + h * D;
-    x[i] = h < heads ? rope_ld<kInterleaved>(base, d) : make_uint4(0, 0, 0, 0);
-  }
-  float c[4], s[4];
+  for (int i = 0; i < kHeads; ++i) x[i] = i < n ? rope_ld<kInterleaved>(src + i * D, d) : make_uint4(0, 0, 0, 0);
+  float c[4], s[4], w[8];
   rope_load(p, d, at, c, s);
+  rope_unpack(rope_ld<kInterleaved>(key ? p.k.weight : p.q.weight, d), w);
   const uint32_t group = kLanes == 32 ? 0xffffffffu
                                       : ((1u << kLanes) - 1u) << ((threadIdx.x & 31) / kLanes * kLanes);
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    if (h >= heads) break;  // the same for the whole group
-    const bool key = h >= p.q.heads;
+    if (i >= n) break;  // the same for the whole group
     float sum = rope_squares(x[i]);
 #pragma unroll
     for (int o = kLanes / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
-    const float r = rsqrtf(sum * (1.0f / D) + p.eps);
-    const uint4 w = rope_ld<kInterleaved>(key ? p.k.weight : p.q.weight, d);
-    __nv_bfloat16* out = key ? p.k.y + (token * p.k.heads + (h - p.q.heads)) * D : p.q.y + (token * p.q.heads + h) * D;
-    rope_store<kInterleaved>(out, d, x[i], w, at < 0 ? __int_as_float(0x7fffffff) : r, c, s);
+    const float r = at < 0 ? __int_as_float(0x7fffffff) : rsqrtf(sum * (1.0f / D) + p.eps);
+    rope_store<kInterleaved>(dst + i * D, d, x[i], w, r, c, s);
   }
 }
 
@@ -190,8 +184,8 @@ __global__ void __launch_bounds__(512) rope_row_kernel(const RopeParams p) {
   __shared__ float part[2][16];
   pdl_wait_prior();
   pdl_launch_dependents();
-  const long long token = blockIdx.x;
-  const int b = int(token / p.rows), t = int(token - (long long)b * p.rows);
+  const int b = blockIdx.y, t = blockIdx.x;
+  const long long token = (long long)b * p.rows + t;
   const RopeDims d = rope_dims<kInterleaved>(threadIdx.x % kLanes, p.pairs);
   const long long at = p.rope ? rope_position(p, b, t) : 0;
   const int heads = p.q.heads + p.k.heads;
@@ -239,7 +233,8 @@ __global__ void __launch_bounds__(512) rope_row_kernel(const RopeParams p) {
     const int h = first + i * step;
     if (h >= heads) break;
     const bool key = h >= p.q.heads;
-    const uint4 w = rope_ld<kInterleaved>(key ? p.k.weight + (h - p.q.heads) * D : p.q.weight + h * D, d);
+    float w[8];
+    rope_unpack(rope_ld<kInterleaved>(key ? p.k.weight + (h - p.q.heads) * D : p.q.weight + h * D, d), w);
     __nv_bfloat16* out = key ? p.k.y + (token * p.k.heads + (h - p.q.heads)) * D : p.q.y + (token * p.q.heads + h) * D;
     rope_store<kInterleaved>(out, d, x[i], w, key ? rk : rq, c, s);
   }

@@ -21,26 +21,24 @@ from waminfer_b200 import _lib
 
 
 def _side(x, weight, heads, name):
+    """Head dim, strides and the operand itself (a copy if the kernel cannot read its rows in place) of q or k."""
     if x.dim() != 3 or x.dtype != torch.bfloat16 or not x.is_cuda:
         raise ValueError(f"{name} must be a bf16 CUDA tensor [batch, rows, heads * head_dim]")
-    if heads < 1 or x.shape[2] % heads:
+    _, rows, width = x.shape
+    if heads < 1 or width % heads:
         raise ValueError(f"{name} {tuple(x.shape)} does not hold {heads} heads")
-    dim = x.shape[2] // heads
-    if weight.dtype != torch.bfloat16 or weight.dim() != 1 or weight.numel() not in (dim, x.shape[2]) \
-            or not weight.is_contiguous() or weight.device != x.device:
-        raise ValueError(f"{name}_weight must be a contiguous bf16 vector of {dim} (each head) or {x.shape[2]} "
+    dim, n = width // heads, weight.numel()
+    if weight.dtype != torch.bfloat16 or weight.dim() != 1 or (n != dim and n != width) or \
+            not weight.is_contiguous() or weight.device != x.device:
+        raise ValueError(f"{name}_weight must be a contiguous bf16 vector of {dim} (each head) or {width} "
                          f"(the row) on {x.device}")
-    return dim
-
-
-def _operand(x):
-    """x with rows the kernel can read in place (any batch stride), else a copy."""
     sb, sr, se = x.stride()
-    if se != 1 or sb % 8 or sr % 8 or x.data_ptr() % 16 or (sr < x.shape[2] and x.shape[1] > 1):
+    if se != 1 or sb % 8 or sr % 8 or x.data_ptr() % 16 or (sr < width and rows > 1):
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x
+        sb, sr, _ = x.stride()
+    return dim, _lib.RowsView(x.data_ptr(), sr, sb), x
 
 
 def _vector(w):
@@ -48,52 +46,58 @@ def _vector(w):
 
 
 def _run(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved):
-    dim = _side(q, q_weight, heads, "q")
-    batch, rows, _ = q.shape
+    dim, q_view, q_held = _side(q, q_weight, heads, "q")
+    batch, rows, width = q.shape
+    device = q.device
     whole = q_weight.numel() != dim
+    k_view, k_at, k_out = _lib.RowsView(), None, None
     if k is not None:
         if k_weight is None:
             raise ValueError("k needs k_weight")
-        if _side(k, k_weight, kv_heads, "k") != dim or k.shape[:2] != q.shape[:2] or k.device != q.device:
+        k_dim, k_view, k_held = _side(k, k_weight, kv_heads, "k")
+        if k_dim != dim or k.shape[:2] != q.shape[:2] or k.device != device:
             raise ValueError(f"q {tuple(q.shape)} ({heads} heads) and k {tuple(k.shape)} ({kv_heads} heads) differ in "
                              "batch, rows, head dim or device")
         whole = whole or k_weight.numel() != dim
-        if whole and (q_weight.numel() != q.shape[2] or k_weight.numel() != k.shape[2]):
+        if whole and (q_weight.numel() != width or k_weight.numel() != k.shape[2]):
             raise ValueError("q_weight and k_weight must both be for each head or both for the row")
-    args = _lib.QkRopeArgs(batch=batch, rows=rows, heads=heads, kv_heads=0 if k is None else kv_heads, head_dim=dim,
-                           whole_row=whole, interleaved=interleaved, eps=eps)
+        k_weight = _vector(k_weight)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_at = k_out.data_ptr()
+    else:
+        kv_heads = 0
+    table = places = None
+    table_stride = table_rows = pairs = place_bytes = place_stride = 0
     if rope is not None:
-        if rope.dtype != torch.complex64 or rope.device != q.device or rope.stride(-1) != 1 or not (
-                rope.dim() == 2 or (rope.dim() == 3 and rope.shape[1] == 1)):
-            raise ValueError(f"rope must be a complex64 table [positions, pairs] (or [positions, 1, pairs]) on {q.device}")
+        shape = rope.shape
+        if rope.dtype != torch.complex64 or rope.device != device or not (
+                len(shape) == 2 or (len(shape) == 3 and shape[1] == 1)) or rope.stride(-1) != 1:
+            raise ValueError(f"rope must be a complex64 table [positions, pairs] (or [positions, 1, pairs]) on {device}")
         if rope.is_conj():
             rope = rope.resolve_conj()
-        if rope.data_ptr() % 16 or rope.stride(0) % 2:
+        table, table_stride, table_rows, pairs = rope.data_ptr(), rope.stride(0), shape[0], shape[-1]
+        if table % 16 or table_stride % 2:
             rope = rope.clone(memory_format=torch.contiguous_format)
-        args.rope, args.table_stride = rope.data_ptr(), rope.stride(0)
-        args.table_rows, args.pairs = rope.shape[0], rope.shape[-1]
+            table, table_stride = rope.data_ptr(), rope.stride(0)
         if positions is not None:
-            if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device or \
-                    tuple(positions.shape) not in ((rows,), (batch, rows)):
-                raise ValueError(f"positions must be int32 or int64, [{rows}] or [{batch}, {rows}], on {q.device}")
-            if positions.stride(-1) != 1 and rows > 1:
+            shape, kind = positions.shape, positions.dtype
+            if (kind != torch.int32 and kind != torch.int64) or positions.device != device or (
+                    shape != (batch, rows) and shape != (rows,)):
+                raise ValueError(f"positions must be int32 or int64, [{rows}] or [{batch}, {rows}], on {device}")
+            if rows > 1 and positions.stride(-1) != 1:
                 positions = positions.contiguous()
-            args.positions, args.position_bytes = positions.data_ptr(), positions.element_size()
-            args.position_stride = positions.stride(0) if positions.dim() == 2 else 0
+            places, place_bytes = positions.data_ptr(), 4 if kind == torch.int32 else 8
+            place_stride = positions.stride(0) if len(shape) == 2 else 0
     elif positions is not None:
         raise ValueError("positions without a rope table")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         return q_out, k_out
-    q, q_weight = _operand(q), _vector(q_weight)
-    args.q = _lib.RowsView(q.data_ptr(), q.stride(1), q.stride(0))
-    args.q_weight, args.q_out = q_weight.data_ptr(), q_out.data_ptr()
-    if k is not None:
-        k, k_weight = _operand(k), _vector(k_weight)
-        args.k = _lib.RowsView(k.data_ptr(), k.stride(1), k.stride(0))
-        args.k_weight, args.k_out = k_weight.data_ptr(), k_out.data_ptr()
-    _lib.launch(_lib.lib().wamffn_qk_norm_rope, q.device.index, ctypes.byref(args))
+    q_weight = _vector(q_weight)
+    args = _lib.QkRopeArgs(q_view, k_view, q_weight.data_ptr(), None if k is None else k_weight.data_ptr(), table,
+                           table_stride, places, place_stride, q_out.data_ptr(), k_at, place_bytes, table_rows, pairs,
+                           batch, rows, heads, kv_heads, dim, whole, interleaved, eps)
+    _lib.launch(_lib.lib().wamffn_qk_norm_rope, device.index, ctypes.byref(args))
     return q_out, k_out
 
 
