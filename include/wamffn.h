@@ -651,17 +651,26 @@ int wamffn_cache_read(void* stream, const wamffn_cache_read_args* args);
  * [g * heads / kv_heads, ...) share key head g.  out contiguous.  fp32 scores,
  * maximum, sums; the probabilities of the value product in f16.  A block id
  * outside the pool is left out and sets WAMFFN_DEV_BAD_INDEX.  key_split: CTAs
- * that share a row tile's keys, 0 picks it (1, 2, 4 or 8 forces it). */
+ * of a cluster that share a row tile's keys, 0 picks it (1, 2, 4 or 8 forces it).
+ * Few row tiles over long sequences are also cut into parts whose shares a second
+ * kernel puts together: workspace (16-byte aligned, the call's own while it runs)
+ * holds them.  Without one, or with fewer bytes than
+ * wamffn_cache_attention_workspace names for the same arguments, the call does
+ * with fewer parts. */
 typedef struct wamffn_cache_attention_args {
   wamffn_cache_view cache;
   wamffn_rows_view q;
   void* out;
+  void* workspace;
+  size_t workspace_bytes;
   int nq;
   int heads;
   int causal;
   int key_split;
 } wamffn_cache_attention_args;
 
+/* Bytes of workspace that the call would like for these arguments (often 0). */
+int wamffn_cache_attention_workspace(const wamffn_cache_attention_args* args, size_t* bytes);
 int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* args);
 
 #ifdef __cplusplus

@@ -289,6 +289,30 @@ def test_attend(cuda_device, batch, nq, heads, kv_heads, lengths, causal):
     assert torch.equal(out, cache.attend(q, heads, causal=causal))  # the same bits again
 
 
+@pytest.mark.parametrize("nq,heads,kv_heads,lengths,causal", [
+    (1, 1, 1, [9000], True), (4, 2, 2, [8200, 10], True), (30, 1, 1, [9000], False), (150, 2, 1, [7000, 0], True),
+    (3, 8, 1, [130, 9001], False)])
+def test_attend_in_parts(cuda_device, nq, heads, kv_heads, lengths, causal):
+    """Few rows over long sequences: parts of the keys through the workspace, some of them empty; and the same
+    call through the C entry without a workspace."""
+    import ctypes
+
+    from waminfer_b200 import _lib
+
+    cache, g = make(cuda_device, nq, len(lengths), kv_heads, lengths, spread=2)
+    q = rows(g, len(lengths), nq, heads * DIM)
+    out = cache.attend(q, heads, causal=causal)
+    assert any(cache._needs.values())  # the call was cut into parts
+    ref = attention(Model(cache), q, heads, causal)
+    close(out, ref, max(lengths))
+    whole = torch.full_like(out, float("nan"))
+    args = _lib.CacheAttentionArgs(cache._view, _lib.RowsView(q.data_ptr(), q.stride(1), q.stride(0)), whole.data_ptr(),
+                                   None, 0, nq, heads, causal, 0)
+    _lib.launch(_lib.lib().wamffn_cache_attention, 0, ctypes.byref(args))
+    close(whole, ref, max(lengths))
+    assert cache.status() == 0
+
+
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 @pytest.mark.parametrize("nq,heads,kv_heads,lengths", [(1, 4, 2, [1000, 40]), (20, 2, 2, [300, 1]), (40, 4, 2, [500, 90])])
 def test_attend_key_split(cuda_device, split, nq, heads, kv_heads, lengths):

@@ -64,7 +64,7 @@ def test_cache_is_checked_by_every_entry(over, code, text):
     view = _lib.RowsView(FAKE, 256, 256)
     for entry, args in ((lib.wamffn_cache_append, _lib.CacheAppendArgs(_cache(**over), view, view, None, None, 1)),
                         (lib.wamffn_cache_read, _lib.CacheReadArgs(_cache(**over), None, FAKE, FAKE, 0, 1)),
-                        (lib.wamffn_cache_attention, _lib.CacheAttentionArgs(_cache(**over), view, FAKE, 1, 2, 0, 0))):
+                        (lib.wamffn_cache_attention, _lib.CacheAttentionArgs(_cache(**over), view, FAKE, None, 0, 1, 2, 0, 0))):
         assert entry(None, ctypes.byref(args)) == code
         assert text in lib.wamffn_last_error()
         assert entry(None, None) == 1
@@ -84,14 +84,24 @@ def test_cache_entries_reject_before_launching():
                        (_lib.CacheReadArgs(_cache(), None, FAKE, None, 0, 1), b"aligned")):
         assert lib.wamffn_cache_read(None, ctypes.byref(args)) == 1
         assert text in lib.wamffn_last_error()
-    for args, text in ((_lib.CacheAttentionArgs(_cache(), view, FAKE, 0, 2, 0, 0), b"nq=0"),
-                       (_lib.CacheAttentionArgs(_cache(), view, FAKE, 1, 3, 0, 0), b"multiple"),
-                       (_lib.CacheAttentionArgs(_cache(), view, FAKE, 1, 2, 0, 3), b"key_split"),
-                       (_lib.CacheAttentionArgs(_cache(), view, FAKE + 4, 1, 2, 0, 0), b"out"),
-                       (_lib.CacheAttentionArgs(_cache(), _lib.RowsView(FAKE + 2, 256, 256), FAKE, 1, 2, 0, 0),
+    for args, text in ((_lib.CacheAttentionArgs(_cache(), view, FAKE, None, 0, 0, 2, 0, 0), b"nq=0"),
+                       (_lib.CacheAttentionArgs(_cache(), view, FAKE, None, 0, 1, 3, 0, 0), b"multiple"),
+                       (_lib.CacheAttentionArgs(_cache(), view, FAKE, None, 0, 1, 2, 0, 3), b"key_split"),
+                       (_lib.CacheAttentionArgs(_cache(), view, FAKE, FAKE + 4, 4096, 1, 2, 0, 0), b"workspace"),
+                       (_lib.CacheAttentionArgs(_cache(), view, FAKE + 4, None, 0, 1, 2, 0, 0), b"out"),
+                       (_lib.CacheAttentionArgs(_cache(), _lib.RowsView(FAKE + 2, 256, 256), FAKE, None, 0, 1, 2, 0, 0),
                         b"aligned")):
         assert lib.wamffn_cache_attention(None, ctypes.byref(args)) == 1
         assert text in lib.wamffn_last_error()
+
+
+def test_workspace_query_rejects_the_same():
+    lib, need = _lib.lib(), ctypes.c_size_t(7)
+    args = _lib.CacheAttentionArgs(_cache(), _lib.RowsView(FAKE, 256, 256), None, None, 0, 1, 3, 0, 0)
+    assert lib.wamffn_cache_attention_workspace(ctypes.byref(args), ctypes.byref(need)) == 1
+    assert b"multiple" in lib.wamffn_last_error() and need.value == 0
+    assert lib.wamffn_cache_attention_workspace(None, ctypes.byref(need)) == 1
+    assert lib.wamffn_cache_attention_workspace(ctypes.byref(args), None) == 1
 
 
 def test_python_refuses_what_it_cannot_run():

@@ -61,6 +61,7 @@ EXPORTED_SYMBOLS = (
     "wamffn_cache_append",
     "wamffn_cache_read",
     "wamffn_cache_attention",
+    "wamffn_cache_attention_workspace",
     "wamffn_rgb_mandatory",
     "wamffn_select_tokens",
     "wamffn_pack_weight",
@@ -216,8 +217,8 @@ class CacheReadArgs(ctypes.Structure):
 class CacheAttentionArgs(ctypes.Structure):
     """Mirror of ``wamffn_cache_attention_args``."""
 
-    _fields_ = [("cache", CacheView), ("q", RowsView), ("out", ctypes.c_void_p), ("nq", ctypes.c_int),
-                ("heads", ctypes.c_int), ("causal", ctypes.c_int), ("key_split", ctypes.c_int)]
+    _fields_ = [("cache", CacheView), ("q", RowsView), ("out", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("nq", ctypes.c_int), ("heads", ctypes.c_int), ("causal", ctypes.c_int), ("key_split", ctypes.c_int)]
 
 
 class BlockArgs(ctypes.Structure):
@@ -342,6 +343,7 @@ def _declare(lib):
     lib.wamffn_cache_append.argtypes = [vp, ctypes.POINTER(CacheAppendArgs)]
     lib.wamffn_cache_read.argtypes = [vp, ctypes.POINTER(CacheReadArgs)]
     lib.wamffn_cache_attention.argtypes = [vp, ctypes.POINTER(CacheAttentionArgs)]
+    lib.wamffn_cache_attention_workspace.argtypes = [ctypes.POINTER(CacheAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
     lib.wamffn_rgb_mandatory.argtypes = [vp, vp, vp, i, i, i, i, vp]
     lib.wamffn_select_tokens.argtypes = [vp, ctypes.POINTER(SelectArgs)]
     lib.wamffn_pack_weight.argtypes = [vp, vp, vp, i, i]

@@ -61,14 +61,14 @@ class KVCache8:
     ``capacity`` rows a sequence; ``blocks`` sizes the pool (default: every
     sequence's full capacity, with a table that gives each its own blocks).  With a
     pool of its own size the caller fills ``block_table`` (int32 [batch, width])
-    before rows reach those places; a block may stand in several tables for reading
+    before rows reach those places; a block may stand in several places for reading
     (a shared prefix), one that rows are appended to in one only.
 
     Tensors: ``keys``, ``values`` [blocks, kv_heads, 64, 128] float8_e4m3fn;
-    ``key_scales``, ``value_scales`` float32 [blocks, kv_heads], powers of two (a
-    row is value * scale); ``block_table``; ``lengths`` int32 [batch], rows held
-    (lowering an entry drops rows).  Calls on one cache follow the stream order of
-    one stream at a time.
+    ``key_scales``, ``value_scales`` float32 [blocks, kv_heads], powers of two from
+    2^-60 (a row is value * scale; of another number only the exponent counts);
+    ``block_table``; ``lengths`` int32 [batch], rows held (lowering an entry drops
+    rows).  Appends to one cache must not overlap in time with other calls on it.
     """
 
     def __init__(self, batch: int, capacity: int, kv_heads: int, device, blocks: int | None = None):
@@ -117,6 +117,7 @@ class KVCache8:
         self.key_scales, self.value_scales = key_scales, value_scales
         self.block_table, self.lengths = block_table, lengths
         self.batch, self.width, self.kv_heads, self.device = batch, width, kv_heads, device
+        self._needs: dict[tuple, int] = {}  # workspace of the attention, by its sizes
         self._work = torch.zeros(batch + 1, dtype=torch.int32, device=device)  # tickets, status word
         self._view = _lib.CacheView(
             keys=keys.data_ptr(), values=values.data_ptr(), key_scales=key_scales.data_ptr(),
@@ -130,7 +131,8 @@ class KVCache8:
         return self.width * BLOCK
 
     def _index(self, name: str, t: torch.Tensor) -> int:
-        _check(name, t, torch.int32, (self.batch,), self.device)
+        if t.dtype != torch.int32 or t.shape != self.lengths.shape or t.device != self.device or not t.is_contiguous():
+            _check(name, t, torch.int32, (self.batch,), self.device)
         return t.data_ptr()
 
     def append(self, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None = None,
@@ -175,9 +177,11 @@ class KVCache8:
         """softmax(q . k / sqrt(128)) . v over each sequence's rows, q [batch,
         nq, heads * 128] bf16, ``heads`` a multiple of ``kv_heads`` (query heads
         [g * heads / kv_heads, ...) share key head g).  ``causal``: the queries
-        are the cache's last nq rows, query i sees rows < length - nq + i + 1.  A
-        row that sees nothing is zeros.  key_split: CTAs sharing a query tile's
-        keys (0 = chosen; 1, 2, 4, 8)."""
+        are the cache's last nq rows, query i sees rows < length - nq + i + 1 (in a
+        ragged batch a sequence with fewer queries has them at the end).  A
+        row that sees nothing is zeros.  NaN comes out where a row sees it: of a
+        query or key in the whole of its heads, of a value in its dim.  key_split:
+        CTAs of a cluster sharing a query tile's keys (0 = chosen; 1, 2, 4, 8)."""
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"heads={heads} must be a multiple of the cache's {self.kv_heads}")
         view, q = _rows(q, "q", self.batch, heads * HEAD_DIM, self.device)
@@ -185,9 +189,25 @@ class KVCache8:
         rows = q.shape[1]
         if rows == 0:
             return out
-        args = _lib.CacheAttentionArgs(self._view, view, out.data_ptr(), rows, heads, causal, key_split)
+        args = _lib.CacheAttentionArgs(self._view, view, out.data_ptr(), None, 0, rows, heads, causal, key_split)
+        held = self._parts(args, rows, heads, key_split)  # kept until the launch, then the stream's
         _lib.launch(_lib.lib().wamffn_cache_attention, self.device.index, ctypes.byref(args))
         return out
+
+    def _parts(self, args, rows: int, heads: int, key_split: int) -> torch.Tensor | None:
+        """Gives the call its workspace; few query rows over a long cache ask for one."""
+        key = (rows, heads, key_split)
+        size = self._needs.get(key)
+        if size is None:
+            need = ctypes.c_size_t()
+            with torch.cuda.device(self.device):
+                _lib.check(_lib.lib().wamffn_cache_attention_workspace(ctypes.byref(args), ctypes.byref(need)))
+            size = self._needs[key] = need.value
+        if not size:
+            return None
+        held = torch.empty(size, dtype=torch.uint8, device=self.device)
+        args.workspace, args.workspace_bytes = held.data_ptr(), size
+        return held
 
     def status(self, clear: bool = True) -> int:
         """Device status word (timeout / bad-index bits); synchronises the device."""

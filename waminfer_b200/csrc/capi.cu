@@ -167,7 +167,8 @@ int prepare_device(int device, int* sm_count) {
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(masked_attention_kernel<true, true>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem));
-    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
     // The kernel's warpgroups trade registers: a split that the launch does not bring would wait for good.
     cudaFuncAttributes many_attr{};
@@ -1904,6 +1905,78 @@ int encode_cache(CUtensorMap* map, const void* base, const CacheView& c, int row
   return WAMFFN_OK;
 }
 
+// Arguments of the attention but for its output.
+int check_cache_attention(const wamffn_cache_attention_args* a, KvAttnParams* p) {
+  if (!a) return fail(WAMFFN_ERR_INVALID, "args is null");
+  int rc = check_cache(a->cache, &p->c);
+  if (rc) return rc;
+  if (a->nq < 1 || a->heads < 1 || a->heads % p->c.kv_heads)
+    return fail(WAMFFN_ERR_INVALID, "nq=%d heads=%d: heads must be a multiple of the cache's %d", a->nq, a->heads,
+                p->c.kv_heads);
+  if (a->key_split != 0 && a->key_split != 1 && a->key_split != 2 && a->key_split != 4 && a->key_split != 8)
+    return fail(WAMFFN_ERR_INVALID, "key_split=%d: 0 (automatic), 1, 2, 4 or 8", a->key_split);
+  if ((rc = check_rows_view(a->q, int64_t(a->heads) * kCacheDim, a->nq, p->c.batch, "q"))) return rc;
+  p->q = static_cast<const __nv_bfloat16*>(a->q.data);
+  p->q_row = a->q.row_stride;
+  p->q_batch = a->q.batch_stride;
+  p->out = static_cast<__nv_bfloat16*>(a->out);
+  p->nq = a->nq;
+  p->heads = a->heads;
+  p->group = a->heads / p->c.kv_heads;
+  p->causal = a->causal != 0;
+  p->scale_log2 = float((1.0 / sqrt(double(kCacheDim))) * 1.4426950408889634);
+  if (int64_t(a->nq) * p->group > 0x7fffffff / 16) return fail(WAMFFN_ERR_INVALID, "too many query rows");
+  return WAMFFN_OK;
+}
+
+// Workspace of one part.
+size_t part_bytes(const KvAttnParams& p) {
+  return size_t(p.c.batch) * p.nq * p.heads * (kCacheDim + 2) * sizeof(float);
+}
+
+// How the keys of a row tile are shared out: `split` CTAs of a cluster (their
+// partial results meet in shared memory, at little cost) and `parts` clusters
+// (whose shares go through the workspace and a second kernel).  The lengths are
+// on the device, so the table's width stands for them.
+struct KvAttnPlan {
+  bool many;
+  int split, parts;
+  int64_t row_tiles;
+};
+
+KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, int most_parts) {
+  const int64_t rows = int64_t(p.nq) * p.group;
+  KvAttnPlan plan{rows > kFewRows, key_split ? key_split : 1, 1, 1};
+  if (plan.many) {
+    // The least waves x (steps of a CTA + what a CTA costs besides, about four steps) + what parts cost, about six;
+    // clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
+    plan.row_tiles = (rows + kManyRows - 1) / kManyRows;
+    const int64_t ctas = plan.row_tiles * p.c.kv_heads * p.c.batch;
+    const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
+    int64_t best = 0;
+    for (int s = 1; s <= 8; ++s) {
+      if (key_split ? s != key_split : 2 * s > std::max<int64_t>(steps, 2)) continue;
+      const int64_t at_once = s == 1 ? sm : many_clusters(s);
+      if (at_once < 1) continue;
+      for (int n = 1; n <= most_parts && (n == 1 || 4 * s * n <= steps); ++n) {
+        const int64_t cost = (ctas * n + at_once - 1) / at_once * ((steps + s * n - 1) / (s * n) + 4) + (n > 1 ? 6 : 0);
+        if (best == 0 || cost < best) best = cost, plan.split = s, plan.parts = n;
+      }
+    }
+    return plan;
+  }
+  // Enough CTAs for three an SM, as long as a warp has a unit; and beyond that as
+  // long as it has sixteen, so that ragged sequences even out over several waves.
+  const int64_t ctas = int64_t(p.c.kv_heads) * p.c.batch, units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys);
+  if (!key_split)
+    for (int s : {2, 4, 8})
+      if (s * kFewWarps * 16 <= units || (ctas * s <= 3 * sm && s * kFewWarps <= units)) plan.split = s;
+  // Parts as long as SMs are left without a CTA and a warp has four units (about what the second kernel costs).
+  const int64_t spare = 3 * int64_t(sm) / (ctas * plan.split), busy = units / (4 * kFewWarps * plan.split);
+  plan.parts = int(std::max<int64_t>(1, std::min<int64_t>(most_parts, std::min(spare, busy))));
+  return plan;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2011,64 +2084,50 @@ int wamffn_cache_read(void* stream, const wamffn_cache_read_args* a) {
   return launch_pdl(cache_read_kernel, dim3(unsigned(ctas), unsigned(p.c.batch)), kReadThreads, 0, 1, stream, p);
 }
 
-int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
-  if (!a) return fail(WAMFFN_ERR_INVALID, "args is null");
+int wamffn_cache_attention_workspace(const wamffn_cache_attention_args* a, size_t* bytes) {
+  if (!bytes) return fail(WAMFFN_ERR_INVALID, "bytes is null");
+  *bytes = 0;
   KvAttnParams p{};
-  int rc = check_cache(a->cache, &p.c);
+  int sm = 0, rc = check_cache_attention(a, &p);
+  if (rc || (rc = prepare_current_device(&sm))) return rc;
+  KvAttnPlan plan = plan_cache_attention(p, a->key_split, sm, 32);
+  if (plan.parts > 1) *bytes = part_bytes(p) * plan.parts;
+  return WAMFFN_OK;
+}
+
+int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
+  KvAttnParams p{};
+  int sm = 0, rc = check_cache_attention(a, &p);
   if (rc) return rc;
-  if (a->nq < 1 || a->heads < 1 || a->heads % p.c.kv_heads)
-    return fail(WAMFFN_ERR_INVALID, "nq=%d heads=%d: heads must be a multiple of the cache's %d", a->nq, a->heads,
-                p.c.kv_heads);
-  if (a->key_split != 0 && a->key_split != 1 && a->key_split != 2 && a->key_split != 4 && a->key_split != 8)
-    return fail(WAMFFN_ERR_INVALID, "key_split=%d: 0 (automatic), 1, 2, 4 or 8", a->key_split);
-  if ((rc = check_rows_view(a->q, int64_t(a->heads) * kCacheDim, a->nq, p.c.batch, "q"))) return rc;
   if (!a->out || !aligned16(a->out)) return fail(WAMFFN_ERR_INVALID, "out must be a 16-byte aligned pointer");
-  p.q = static_cast<const __nv_bfloat16*>(a->q.data);
-  p.q_row = a->q.row_stride;
-  p.q_batch = a->q.batch_stride;
-  p.out = static_cast<__nv_bfloat16*>(a->out);
-  p.nq = a->nq;
-  p.heads = a->heads;
-  p.group = a->heads / p.c.kv_heads;
-  p.causal = a->causal != 0;
-  p.scale_log2 = float((1.0 / sqrt(double(kCacheDim))) * 1.4426950408889634);
-  const int64_t rows = int64_t(a->nq) * p.group;
-  if (rows > 0x7fffffff / 16) return fail(WAMFFN_ERR_INVALID, "too many query rows");
-  int sm = 0;
+  if (a->workspace && !aligned16(a->workspace))
+    return fail(WAMFFN_ERR_INVALID, "workspace must be a 16-byte aligned pointer");
   if ((rc = prepare_current_device(&sm))) return rc;
-  if (rows > kFewRows) {
-    const int64_t row_tiles = (rows + kManyRows - 1) / kManyRows, ctas = row_tiles * p.c.kv_heads * p.c.batch;
-    // Key split: the one with the least waves x (steps of a CTA + what a CTA costs besides, about four steps);
-    // clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
-    const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
-    p.split = a->key_split ? a->key_split : 1;
-    if (!a->key_split) {
-      int64_t best = 0;
-      for (int s = 1; s <= 8 && 2 * s <= std::max<int64_t>(steps, 2); ++s) {
-        const int64_t at_once = s == 1 ? sm : many_clusters(s);
-        if (at_once < 1) continue;
-        const int64_t cost = (ctas + at_once - 1) / at_once * ((steps + s - 1) / s + 4);
-        if (best == 0 || cost < best) best = cost, p.split = s;
-      }
-    }
-    if (row_tiles * p.split > 0x7fffffff) return fail(WAMFFN_ERR_INVALID, "too many query rows");
-    return launch_pdl(kv_attend_many_kernel, dim3(unsigned(row_tiles * p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
-                      kManyThreads, kManySmem, p.split, stream, p);
+  const size_t part = part_bytes(p);
+  const int most = a->workspace ? int(std::min<size_t>(a->workspace_bytes / part, 32)) : 1;
+  const KvAttnPlan plan = plan_cache_attention(p, a->key_split, sm, most);
+  p.split = plan.split;
+  p.parts = plan.parts;
+  const int64_t rows = int64_t(p.c.batch) * p.nq * p.heads;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + size_t(plan.parts) * rows * kCacheDim);
+  const int64_t x = plan.row_tiles * plan.split * plan.parts;
+  if (x > 0x7fffffff || (plan.parts > 1 && rows > 0x7fffffff))
+    return fail(WAMFFN_ERR_INVALID, "too many query rows");
+  const dim3 grid(unsigned(x), unsigned(p.c.kv_heads), unsigned(p.c.batch));
+  if (plan.many) {
+    rc = launch_pdl(kv_attend_many_kernel, grid, kManyThreads, kManySmem, p.split, stream, p);
+  } else {
+    CUtensorMap kmap, vmap;
+    if ((rc = encode_cache(&kmap, p.c.keys, p.c, kUnitKeys))) return rc;
+    if ((rc = encode_cache(&vmap, p.c.values, p.c, kUnitKeys))) return rc;
+    auto kernel = int64_t(p.nq) * p.group <= 8 ? kv_attend_few_kernel<true> : kv_attend_few_kernel<false>;
+    rc = launch_pdl(kernel, grid, kFewWarps * 32, kFewSmem, p.split, stream, kmap, vmap, p);
   }
-  // Key split: enough CTAs for three an SM, as long as a warp has a unit; and beyond that as long as it has
-  // sixteen, so that ragged sequences even out over several waves.
-  const int64_t ctas = int64_t(p.c.kv_heads) * p.c.batch, units = int64_t(p.c.width) * (kCacheBlock / kUnitKeys);
-  p.split = 1;
-  if (a->key_split)
-    p.split = a->key_split;
-  else
-    for (int s : {2, 4, 8})
-      if (s * kFewWarps * 16 <= units || (ctas * s <= 3 * sm && s * kFewWarps <= units)) p.split = s;
-  CUtensorMap kmap, vmap;
-  if ((rc = encode_cache(&kmap, p.c.keys, p.c, kUnitKeys))) return rc;
-  if ((rc = encode_cache(&vmap, p.c.values, p.c, kUnitKeys))) return rc;
-  return launch_pdl(kv_attend_few_kernel, dim3(unsigned(p.split), unsigned(p.c.kv_heads), unsigned(p.c.batch)),
-                    kFewWarps * 32, kFewSmem, p.split, stream, kmap, vmap, p);
+  if (rc || plan.parts == 1) return rc;
+  constexpr int per = kMergeThreads / 32;
+  return launch_pdl(kv_merge_kernel, dim3(unsigned((rows + per - 1) / per)), kMergeThreads, 0, 1, stream, p,
+                    (long long)rows);
 }
 
 }  // extern "C"

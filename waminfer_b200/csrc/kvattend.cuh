@@ -35,8 +35,51 @@ struct KvAttnParams {
   long long q_row, q_batch;  // strides, elements
   __nv_bfloat16* out;        // [batch, nq, heads 128]
   int nq, heads, group, causal, split;
+  int parts;                 // of the keys, each with a cluster of its own
+  float* part_o;             // parts > 1: unnormalised rows [parts, batch, nq, heads, 128]
+  float2* part_ml;           // and their (maximum, normaliser) [parts, batch, nq, heads]
   float scale_log2;          // log2(e) / sqrt(128)
 };
+
+// Four dims of a row: the result, or with parts this part's share of it.
+__device__ __forceinline__ void kv_emit(const KvAttnParams& p, int part, int b, int token, int head, int d,
+                                        const float4& v, float top, float sum) {
+  const size_t row = (size_t(b) * p.nq + token) * p.heads + head;
+  if (p.parts == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // nothing seen: zeros
+    *reinterpret_cast<uint2*>(p.out + row * kCacheDim + d) =
+        make_uint2(bf2_pack(v.x * inv, v.y * inv), bf2_pack(v.z * inv, v.w * inv));
+  } else {
+    const size_t at = size_t(part) * p.c.batch * p.nq * p.heads + row;
+    *reinterpret_cast<float4*>(p.part_o + at * kCacheDim + d) = v;
+    if (d == 0) p.part_ml[at] = make_float2(top, sum);
+  }
+}
+
+// The parts' shares of a row in their order; a warp a row.
+constexpr int kMergeThreads = 256;
+__global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvAttnParams p, long long rows) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const long long row = (long long)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int d = (threadIdx.x & 31) * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = -INFINITY, sum = 0.f;
+  for (int k = 0; k < p.parts; ++k) {
+    const float2 ml = p.part_ml[k * rows + row];
+    const float4 u = *reinterpret_cast<const float4*>(p.part_o + (k * rows + row) * kCacheDim + d);
+    const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
+    const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
+    v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
+    v.z = v.z * fo + u.z * fn, v.w = v.w * fo + u.w * fn;
+    sum = sum * fo + ml.y * fn;
+    top = next;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(p.out + row * kCacheDim + d) =
+      make_uint2(bf2_pack(v.x * inv, v.y * inv), bf2_pack(v.z * inv, v.w * inv));
+}
 
 constexpr float kPBias = 5.f, kLag = 8.f;  // P <= 2^(5 + 8)
 
@@ -51,6 +94,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Transposes an 8 x 8 matrix of f16 held two a lane (row lane / 4, columns 2 (lane % 4) ..).
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -129,10 +179,12 @@ __device__ __forceinline__ uint4 clean_chunk(uint4 u, int key, int length, bool 
 // into a ring; the fragments are converted in registers (a lane takes 16
 // neighbouring dims of K, which the product's order of k allows, and the same
 // 16 dims of four rows of V), so nothing is written back to shared memory.
-// Four warps with rings and units of their own, three CTAs an SM (168 registers:
-// a unit is one long chain of dependent steps, and warps hide each other's);
-// a cluster of `split` CTAs shares the keys, and the partial results meet through
-// distributed shared memory.
+// Up to 8 rows stand as the products' columns (S^T = K Q^T, O^T = V^T P^T: half the
+// instructions of rows as rows, 32 instead of 64 accumulators), up to 16 as their rows.
+// Four warps with rings and units of their own, three CTAs an SM (a unit is one
+// long chain of dependent steps, and warps hide each other's);
+// a cluster of `split` CTAs shares the keys of a part, and the partial results meet
+// through distributed shared memory.
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 16;  // packed rows of a key head at most; beyond, kvattend_many.cuh
 constexpr int kUnitKeys = 32;
@@ -144,6 +196,7 @@ constexpr int kFewRing = kFewStages * 2 * kUnitBytes;  // of a warp
 constexpr int kFewSmem = kFewWarps * kFewRing + 1024;
 static_assert(kFewRows * kFewPitch * 4 <= kFewRing, "a partial result fits its warp's ring");
 
+template <bool kNarrow>
 __global__ void __launch_bounds__(kFewWarps * 32, 3)
     kv_attend_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                          const KvAttnParams p) {
@@ -158,7 +211,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int split = p.split, rank = blockIdx.x;
+  const int split = p.split, part = int(blockIdx.x) / split, rank = int(blockIdx.x) - part * split;
   const int kh = blockIdx.y, b = blockIdx.z;
 
   if (threadIdx.x == 0) {
@@ -175,7 +228,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
   pdl_launch_dependents();
 
   const CacheView& c = p.c;
-  const int worker = rank * kFewWarps + warp, workers = split * kFewWarps;
+  const int worker = int(blockIdx.x) * kFewWarps + warp, workers = int(gridDim.x) * kFewWarps;
   uint8_t* my_ring = ring + warp * kFewRing;
   uint64_t* my_full = full[warp];
   // Block ids and scales of 32 of this warp's units (worker + i * workers) at a time, one a lane.  The scales are
@@ -230,19 +283,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
   };
   for (int i = 0; i < min(mine, kFewStages); ++i) issue(i);
 
-  // Query fragments: rows g and g + 8 of the warp's tile, dims [32 t, 32 t + 32):
-  // step ks = 4 c + w takes dims 32 t + 16 c + 4 w + {0, 1} and {2, 3} as its k
-  // columns 2 t, 2 t + 1 and 2 t + 8, 2 t + 9.
-  uint32_t qa[8][4];
-  float qf[2];      // 2^eq log2(e) / sqrt(128) of the rows
-  int seen[2];
+  // Query fragments, dims [32 t, 32 t + 32) of row g (and of row g + 8 unless narrow): step ks = 4 c + w takes dims
+  // 32 t + 16 c + 4 w + {0, 1} and {2, 3} as its k columns 2 t, 2 t + 1 and 2 t + 8, 2 t + 9.
+  constexpr int kHalves = kNarrow ? 1 : 2;
+  uint32_t qa[8][2 * kHalves];
+  float qf[2];      // 2^eq log2(e) / sqrt(128) of the lane's rows: 2 t, 2 t + 1 if narrow, else g, g + 8
+  int seen[2];      // keys that these see
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < kHalves; ++half) {
     const int r = g + 8 * half;
     const bool live = r < rows;
     const int token = live ? r / p.group : 0;
     const int head = kh * p.group + (live ? r - token * p.group : 0);
-    seen[half] = live ? keys_seen(length, p.nq, token, p.causal) : 0;
     const __nv_bfloat16* src = p.q + b * p.q_batch + token * p.q_row + size_t(head) * kCacheDim + 32 * t;
     uint4 u[4];
     float top = 0.f;
@@ -263,11 +315,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
       const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)  // words 4 i + e: dims 32 t + 8 i + 2 e; step 2 i + e / 2, column pair e % 2
-        qa[2 * i + (e >> 1)][half + 2 * (e & 1)] = f16x2_pack(bf2_lo(w[e]) * inv, bf2_hi(w[e]) * inv);
+        qa[2 * i + (e >> 1)][half + kHalves * (e & 1)] = f16x2_pack(bf2_lo(w[e]) * inv, bf2_hi(w[e]) * inv);
     }
   }
+  if constexpr (kNarrow) {
+    const float mine_qf = qf[0];
+    qf[0] = __shfl_sync(0xffffffffu, mine_qf, 8 * t);
+    qf[1] = __shfl_sync(0xffffffffu, mine_qf, 8 * t + 4);
+  }
+  auto row_of = [&](int i) { return kNarrow ? 2 * t + i : g + 8 * i; };  // the lane's two rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    seen[i] = row_of(i) < rows ? keys_seen(length, p.nq, row_of(i) / p.group, p.causal) : 0;
 
-  float o[16][4] = {};
+  // Narrow: o[i] = dims 16 g + 2 i (+ 1 in the upper two) of rows 2 t, 2 t + 1; else o[n] = dims 32 t + n (+ 16) of
+  // rows g, g + 8.
+  float o[kNarrow ? 8 : 16][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   Info now = ahead;
   int now_chunk = 0;
@@ -287,22 +350,34 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
     if (id >= 0) {
       const int key0 = (worker + i * workers) * kUnitKeys;
       const uint32_t kb = smem_addr(my_ring + s * 2 * kUnitBytes), vb = kb + kUnitBytes;
-      // S = Q K^T, 8 keys a tile; the four tiles' sums advance together.
-      float x[4][4] = {};
+      // S: x[j][e] is row row_of(e & 1) (narrow) or row_of(e >> 1), key 16 j + g + 8 (e >> 1) (narrow) or
+      // 8 j + 2 t + (e & 1).  The tiles' sums advance together.
+      constexpr int kTiles = kNarrow ? 2 : 4;
+      float x[kTiles][4] = {};
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc) {
-        uint32_t w[4][4];
+        uint32_t w[4][4];  // keys 8 j + g, 16 dims
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const uint4 u = lds128(kb + (nt * 8 + g) * kCacheDim + (((2 * t + cc) ^ g) << 4));
-          w[nt][0] = u.x, w[nt][1] = u.y, w[nt][2] = u.z, w[nt][3] = u.w;
+        for (int j = 0; j < 4; ++j) {
+          const uint4 u = lds128(kb + (j * 8 + g) * kCacheDim + (((2 * t + cc) ^ g) << 4));
+          w[j][0] = u.x, w[j][1] = u.y, w[j][2] = u.z, w[j][3] = u.w;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt)
-            mma_f16(x[nt], qa[cc * 4 + e], e4m3x2_to_f16x2(w[nt][e]), e4m3x2_hi_to_f16x2(w[nt][e]));
+          for (int j = 0; j < kTiles; ++j) {
+            const uint32_t* q = qa[cc * 4 + e];
+            if constexpr (kNarrow) {
+              const uint32_t ka[4] = {e4m3x2_to_f16x2(w[2 * j][e]), e4m3x2_to_f16x2(w[2 * j + 1][e]),
+                                      e4m3x2_hi_to_f16x2(w[2 * j][e]), e4m3x2_hi_to_f16x2(w[2 * j + 1][e])};
+              mma_f16(x[j], ka, q[0], q[1]);
+            } else {
+              const uint32_t a[4] = {q[0], q[1], q[2], q[3]};
+              mma_f16(x[j], a, e4m3x2_to_f16x2(w[j][e]), e4m3x2_hi_to_f16x2(w[j][e]));
+            }
+          }
       }
+      auto slot = [](int e) { return kNarrow ? e & 1 : e >> 1; };  // which of the lane's rows x[.][e] belongs to
       const bool whole = key0 + kUnitKeys <= least;  // every row sees every key of the unit
       if (!whole) {
         // Keys that every row sees need no look.
@@ -316,23 +391,25 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
         fence_proxy_async();  // the place is refilled by a bulk copy
         __syncwarp();
       }
-      const float f0 = qf[0] * kf, f1 = qf[1] * kf, evf = float(ev);
+      const float f[2] = {qf[0] * kf, qf[1] * kf}, evf = float(ev);
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int j = 0; j < kTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = fmaf(x[nt][e], (e >> 1) ? f1 : f0, evf);
-          if (!whole && key0 + nt * 8 + 2 * t + (e & 1) >= seen[e >> 1]) v = -INFINITY;
-          x[nt][e] = v;
-          top[e >> 1] = fmaxf(top[e >> 1], v);
+          float v = fmaf(x[j][e], f[slot(e)], evf);
+          const int key = key0 + (kNarrow ? 16 * j + g + 8 * (e >> 1) : 8 * j + 2 * t + (e & 1));
+          if (!whole && key >= seen[slot(e)]) v = -INFINITY;
+          x[j][e] = v;
+          top[slot(e)] = fmaxf(top[slot(e)], v);
         }
       float base[2], corr[2];
       bool grown = false;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-        top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+#pragma unroll
+        for (int w = kNarrow ? 4 : 1; w < (kNarrow ? 32 : 4); w <<= 1)
+          top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], w));
         // A maximum that grows by at most 2^kLag is left as it is: P stays below f16's range.
         const bool g = top[half] > m[half] + kLag || (m[half] == -INFINITY && top[half] > m[half]);
         corr[half] = g ? ex2_approx(m[half] - top[half]) : 1.f;
@@ -342,28 +419,32 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
       }
       float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      for (int j = 0; j < kTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[nt][e] = ex2_approx(x[nt][e] + base[e >> 1]);
-          sum[e >> 1] += x[nt][e];
+          x[j][e] = ex2_approx(x[j][e] + base[slot(e)]);
+          sum[slot(e)] += x[j][e];
         }
       const float back = exp2_int(-ev);
       l[0] = fmaf(sum[0], back, l[0] * corr[0]);
       l[1] = fmaf(sum[1], back, l[1] * corr[1]);
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          o[n][0] *= corr[0], o[n][1] *= corr[0];
-          o[n][2] *= corr[1], o[n][3] *= corr[1];
-        }
+        for (int n = 0; n < (kNarrow ? 8 : 16); ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][e] *= corr[slot(e)];
       }
-      // O += P V, 16 keys a step; tile n holds dims 16 g' + n (g' the tile's column).
+      // O += P V, 16 keys a step.
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        const uint32_t pa[4] = {f16x2_pack(x[2 * ks][0], x[2 * ks][1]), f16x2_pack(x[2 * ks][2], x[2 * ks][3]),
-                                f16x2_pack(x[2 * ks + 1][0], x[2 * ks + 1][1]),
-                                f16x2_pack(x[2 * ks + 1][2], x[2 * ks + 1][3])};
+        uint32_t pa[4];
+        if constexpr (kNarrow) {  // keys x rows to rows x keys
+          pa[0] = transpose8(f16x2_pack(x[ks][0], x[ks][1]));
+          pa[1] = transpose8(f16x2_pack(x[ks][2], x[ks][3]));
+        } else {
+          pa[0] = f16x2_pack(x[2 * ks][0], x[2 * ks][1]), pa[1] = f16x2_pack(x[2 * ks][2], x[2 * ks][3]);
+          pa[2] = f16x2_pack(x[2 * ks + 1][0], x[2 * ks + 1][1]), pa[3] = f16x2_pack(x[2 * ks + 1][2], x[2 * ks + 1][3]);
+        }
         uint32_t w[4][4];  // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the step, dims [16 g, 16 g + 16)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -375,10 +456,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
         for (int e = 0; e < 4; ++e) {
           const uint32_t a = __byte_perm(w[0][e], w[1][e], 0x5140), z = __byte_perm(w[2][e], w[3][e], 0x5140);
           const uint32_t a2 = __byte_perm(w[0][e], w[1][e], 0x7362), z2 = __byte_perm(w[2][e], w[3][e], 0x7362);
-          mma_f16(o[4 * e], pa, e4m3x2_to_f16x2(a), e4m3x2_to_f16x2(z));
-          mma_f16(o[4 * e + 1], pa, e4m3x2_hi_to_f16x2(a), e4m3x2_hi_to_f16x2(z));
-          mma_f16(o[4 * e + 2], pa, e4m3x2_to_f16x2(a2), e4m3x2_to_f16x2(z2));
-          mma_f16(o[4 * e + 3], pa, e4m3x2_hi_to_f16x2(a2), e4m3x2_hi_to_f16x2(z2));
+          if constexpr (kNarrow) {
+            const uint32_t v0[4] = {e4m3x2_to_f16x2(a), e4m3x2_hi_to_f16x2(a), e4m3x2_to_f16x2(z), e4m3x2_hi_to_f16x2(z)};
+            const uint32_t v1[4] = {e4m3x2_to_f16x2(a2), e4m3x2_hi_to_f16x2(a2), e4m3x2_to_f16x2(z2),
+                                    e4m3x2_hi_to_f16x2(z2)};
+            mma_f16(o[2 * e], v0, pa[0], pa[1]);
+            mma_f16(o[2 * e + 1], v1, pa[0], pa[1]);
+          } else {
+            mma_f16(o[4 * e], pa, e4m3x2_to_f16x2(a), e4m3x2_to_f16x2(z));
+            mma_f16(o[4 * e + 1], pa, e4m3x2_hi_to_f16x2(a), e4m3x2_hi_to_f16x2(z));
+            mma_f16(o[4 * e + 2], pa, e4m3x2_to_f16x2(a2), e4m3x2_to_f16x2(z2));
+            mma_f16(o[4 * e + 3], pa, e4m3x2_hi_to_f16x2(a2), e4m3x2_hi_to_f16x2(z2));
+          }
         }
       }
     }
@@ -389,20 +478,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
     for (int i = max(0, issued - kFewStages); i < issued; ++i)
       wait_drain(smem_addr(&my_full[i % kFewStages]), uint32_t(i / kFewStages) & 1u);
   __syncthreads();  // every ring is idle: partial results go over them
-  float* part = reinterpret_cast<float*>(my_ring);
+  float* held = reinterpret_cast<float*>(my_ring);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-    l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-    const int r = g + 8 * half;
-    if (t == 0) part_ml[warp][r] = make_float2(m[half], l[half]);
 #pragma unroll
-    for (int n = 0; n < 16; n += 4)
+    for (int w = kNarrow ? 4 : 1; w < (kNarrow ? 32 : 4); w <<= 1) l[half] += __shfl_xor_sync(0xffffffffu, l[half], w);
+    const int r = row_of(half);
+    if ((kNarrow ? g : t) == 0) part_ml[warp][r] = make_float2(m[half], l[half]);
 #pragma unroll
-      for (int col = 0; col < 2; ++col) {  // column 2 t + col of tiles n .. n + 3: dims 32 t + 16 col + n
-        const int dim = 32 * t + 16 * col + n;
-        float4 v = make_float4(o[n][2 * half + col], o[n + 1][2 * half + col], o[n + 2][2 * half + col],
-                               o[n + 3][2 * half + col]);
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int col = 0; col < (kNarrow ? 1 : 2); ++col) {  // four neighbouring dims
+        const int dim = kNarrow ? 16 * g + 4 * n : 32 * t + 16 * col + 4 * n;
+        float4 v;
+        if constexpr (kNarrow)
+          v = make_float4(o[2 * n][half], o[2 * n][2 + half], o[2 * n + 1][half], o[2 * n + 1][2 + half]);
+        else
+          v = make_float4(o[4 * n][2 * half + col], o[4 * n + 1][2 * half + col], o[4 * n + 2][2 * half + col],
+                          o[4 * n + 3][2 * half + col]);
         if (nan_any) {
           const float bad = __int_as_float(0x7fffffff);
           if (nan_key[dim] < seen[half]) v.x = bad;
@@ -410,7 +503,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
           if (nan_key[dim + 2] < seen[half]) v.z = bad;
           if (nan_key[dim + 3] < seen[half]) v.w = bad;
         }
-        *reinterpret_cast<float4*>(part + r * kFewPitch + dim) = v;
+        *reinterpret_cast<float4*>(held + r * kFewPitch + dim) = v;
       }
   }
   __syncthreads();
@@ -466,11 +559,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
       v.x += u[k].x * f, v.y += u[k].y * f, v.z += u[k].z * f, v.w += u[k].w * f;
       sum += ml[k].y * f;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // nothing seen: zeros
     const int token = r / p.group, head = kh * p.group + r - token * p.group;
-    if (!abort_flag)
-      *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.nq + token) * p.heads + head) * kCacheDim + d) =
-          make_uint2(bf2_pack(v.x * inv, v.y * inv), bf2_pack(v.z * inv, v.w * inv));
+    if (!abort_flag) kv_emit(p, part, b, token, head, d, v, top, sum);
   }
   if (split > 1) cluster_sync();  // no CTA leaves while a peer reads its shared memory
 }

@@ -22,8 +22,8 @@
 //   warps 0, 1      one thread a tile issues S = Q K^T and O += P V; warps 2 and 3 are idle
 //
 // TMEM: S of tile x, step j at 128 x + 64 (j & 1), O of tile x at 256 + 128 x.
-// `split` CTAs of a cluster share a row tile's steps and meet through distributed
-// shared memory.  Every wait is bounded in time and raises WAMFFN_DEV_TIMEOUT.
+// `split` CTAs of a cluster share a row tile's steps (of a part) and meet through
+// distributed shared memory.  Every wait is bounded in time and raises WAMFFN_DEV_TIMEOUT.
 // The loops are kept small (one copy of each, rare paths not unrolled): all roles
 // share the instruction cache.
 #pragma once
@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.split, kh = blockIdx.y, b = blockIdx.z;
   // The last row tile first: with a causal mask it has the most keys.
-  const int tile = int(gridDim.x / split) - 1 - int(blockIdx.x) / split, rank = int(blockIdx.x) % split;
+  const int shares = split * p.parts, share = int(blockIdx.x) % shares;  // of the keys: rank of the cluster in its part
+  const int tile = int(gridDim.x) / shares - 1 - int(blockIdx.x) / shares, rank = share % split, part = share / split;
   const int total_rows = p.nq * p.group, row0 = tile * kManyRows;
   const int rows = min(kManyRows, total_rows - row0);
   const bool dual = rows <= 128;  // both tiles hold the same rows and take every second step
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   const int least = keys_seen(length, p.nq, row0 / p.group, p.causal);
   const int most = keys_seen(length, p.nq, (row0 + rows - 1) / p.group, p.causal);
   const int all_steps = (most + kManyStep - 1) / kManyStep;
-  const int first = int((long long)rank * all_steps / split);
-  const int steps = int((long long)(rank + 1) * all_steps / split) - first;
+  const int first = int((long long)share * all_steps / shares);
+  const int steps = int((long long)(share + 1) * all_steps / shares) - first;
 
   if (warp < kManyConvWarp0) {
     // ------------------------------------------------------------ products
@@ -476,7 +477,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         for (int q = 0; q < 4; ++q) {
           uint32_t v[32];
           load_o(q, v);
-          if (live)
+          if (live && p.parts > 1) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              kv_emit(p, part, b, token, head, q * 32 + i,
+                      make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]),
+                                  __uint_as_float(v[i + 3])), m, l);
+          } else if (live) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               float o[8];
@@ -485,14 +492,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
               *reinterpret_cast<uint4*>(dst + q * 32 + i) =
                   make_uint4(bf2_pack(o[0], o[1]), bf2_pack(o[2], o[3]), bf2_pack(o[4], o[5]), bf2_pack(o[6], o[7]));
             }
+          }
         }
       }
     } else {
       // This CTA's partial rows (unnormalised O, maximum, normaliser) to shared memory; every product has read it.
-      float* part = reinterpret_cast<float*>(smem);
-      float2* part_ml = reinterpret_cast<float2*>(part + kManyRows * kManyPitch);
+      float* held = reinterpret_cast<float*>(smem);
+      float2* held_ml = reinterpret_cast<float2*>(held + kManyRows * kManyPitch);
       if (live) {
-        part_ml[r] = make_float2(m, l);
+        held_ml[r] = make_float2(m, l);
       }
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {
@@ -501,7 +509,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         if (live)
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + r * kManyPitch + q * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            *reinterpret_cast<uint4*>(held + r * kManyPitch + q * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       }
       __syncwarp();
       cluster_sync();
@@ -513,8 +521,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         float top = -INFINITY, sum = 0.f;
         for (int k = 0; k < split * stride; ++k) {  // CTA, and tile where both hold the row
           const int from = dual ? k >> 1 : k, at = pr + (dual ? 128 * (k & 1) : 0);
-          const float2 ml = ld_cluster2(map_to_cta(smem_addr(&part_ml[at]), from));
-          const float4 u = ld_cluster4(map_to_cta(smem_addr(part + at * kManyPitch + d), from));
+          const float2 ml = ld_cluster2(map_to_cta(smem_addr(&held_ml[at]), from));
+          const float4 u = ld_cluster4(map_to_cta(smem_addr(held + at * kManyPitch + d), from));
           const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
           const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
           v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
@@ -522,11 +530,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           sum = sum * fo + ml.y * fn;
           top = next;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int prow = row0 + pr, ptoken = prow / p.group, phead = kh * p.group + prow - ptoken * p.group;
-        if (!*abort)
-          *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.nq + ptoken) * p.heads + phead) * kCacheDim + d) =
-              make_uint2(bf2_pack(v.x * inv, v.y * inv), bf2_pack(v.z * inv, v.w * inv));
+        if (!*abort) kv_emit(p, part, b, ptoken, phead, d, v, top, sum);
       }
       __syncwarp();
       cluster_sync();  // no CTA leaves while a peer reads its shared memory

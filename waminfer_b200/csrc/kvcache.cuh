@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kReadThreads) cache_read_kernel(const CacheRea
     const int id = c.table[b * c.table_stride + row / kCacheBlock];
     if (id >= 0 && id < c.blocks) {
       const size_t tile = size_t(id) * c.kv_heads + h;
-      const float s = (value ? c.value_scales : c.key_scales)[tile];
+      const float s = exp2_int(scale_exp((value ? c.value_scales : c.key_scales)[tile]));
       const uint4 u = *reinterpret_cast<const uint4*>((value ? c.values : c.keys) + tile * kCacheTile +
                                                       (row % kCacheBlock) * kCacheDim + lane * 16);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
