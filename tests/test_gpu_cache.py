@@ -480,6 +480,32 @@ def test_a_decode_run(cuda_device):
     assert cache.status() == 0
 
 
+def test_traced(cuda_device):
+    """The calls inside a compiled function: the same cache and results as called one by one."""
+    from waminfer_b200.cache import KVCache8
+    from waminfer_b200.rope import qk_norm_rope
+
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    qkv, w = rows(g, 2, 5, 4 * DIM), rows(g, DIM)
+    freqs = torch.polar(torch.ones(8, 64), torch.rand(8, 64)).to(cuda_device)
+    caches = [KVCache8(2, 128, 1, cuda_device) for _ in range(2)]
+    at = torch.tensor([0, 0], dtype=torch.int32, device=cuda_device)
+
+    def step(cache, qkv):
+        q, k, v = qkv.split([2 * DIM, DIM, DIM], -1)
+        q, k = qk_norm_rope(q, k, w, w, freqs, None, 2, 1)
+        cache.append(k, v, at=at)
+        return cache.attend(q, 2, causal=True) * 1.0, *cache.read(5), *cache.read(3, start=at)
+
+    with torch.no_grad():
+        plain = step(caches[0], qkv)
+        traced = torch.compile(lambda qkv: step(caches[1], qkv), backend="aot_eager", fullgraph=True)(qkv)
+    for a, b in zip(plain, traced):
+        assert torch.equal(a, b)
+    assert torch.equal(caches[0].lengths, caches[1].lengths) and torch.equal(caches[0].keys.view(torch.uint8),
+                                                                             caches[1].keys.view(torch.uint8))
+
+
 def test_two_graphs_and_two_caches_at_once(cuda_device):
     """Two captured attention steps over different caches, replayed on two streams at the same time."""
     made = [make(cuda_device, i, 2, 4, [900 + 50 * i, 300], spread=1) for i in range(2)]

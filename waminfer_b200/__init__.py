@@ -16,6 +16,10 @@ Modules mirror the reference's host interface for the path:
   across the ranks of a process group (one all-reduce per layer);
 * ``waminfer_b200.euler``   -- the 10-update Euler schedule over the stack;
 * ``waminfer_b200.projections`` -- attention-side projections on the same GEMM;
+* ``waminfer_b200.rope``    -- norm of queries and keys with the rotation in one
+  pass, between the projections and the attention;
+* ``waminfer_b200.cache``   -- keys and values in 8 bits (``KVCache8``): store,
+  attention over them, rows back as bf16;
 * ``waminfer_b200.trace``   -- per-CTA phase timelines of the library's kernels.
 
 All GPU work runs in ``libwamffn.so`` (``waminfer_b200/csrc``); importing an op

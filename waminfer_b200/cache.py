@@ -55,6 +55,57 @@ def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device:
                          f"{t.dtype} {list(t.shape)} on {t.device}")
 
 
+def _layout(keys, values, key_scales, value_scales, block_table, lengths, work) -> _lib.CacheView:
+    """The C view of a cache's tensors; work: [batch] tickets and the status word."""
+    (pool, kv_heads), (batch, width) = keys.shape[:2], block_table.shape
+    return _lib.CacheView(
+        keys=keys.data_ptr(), values=values.data_ptr(), key_scales=key_scales.data_ptr(),
+        value_scales=value_scales.data_ptr(), block_table=block_table.data_ptr(), table_stride=width,
+        lengths=lengths.data_ptr(), tickets=work.data_ptr(), status=work.data_ptr() + 4 * batch,
+        blocks=pool, kv_heads=kv_heads, batch=batch, width=width)
+
+
+# The calls as ops on the cache's tensors, for traced code (the methods call the library directly otherwise).
+@torch.library.custom_op("wam_ffn::cache_append", mutates_args=("keys", "values", "key_scales", "value_scales",
+                                                                "lengths", "work"))
+def _append_op(k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None, at: torch.Tensor | None,
+               keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+               block_table: torch.Tensor, lengths: torch.Tensor, work: torch.Tensor) -> None:
+    KVCache8._of(keys, values, key_scales, value_scales, block_table, lengths, work)._append(k, v, counts, at)
+
+
+@_append_op.register_fake
+def _append_fake(k, v, counts, at, keys, values, key_scales, value_scales, block_table, lengths, work):
+    return None
+
+
+@torch.library.custom_op("wam_ffn::cache_read", mutates_args=("work",))
+def _read_op(count: int, start: torch.Tensor | None, start_all: int, keys: torch.Tensor, values: torch.Tensor,
+             key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+             work: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    cache = KVCache8._of(keys, values, key_scales, value_scales, block_table, lengths, work)
+    return cache._read(count, start_all if start is None else start)
+
+
+@_read_op.register_fake
+def _read_fake(count, start, start_all, keys, values, key_scales, value_scales, block_table, lengths, work):
+    shape = (block_table.shape[0], count, keys.shape[1] * HEAD_DIM)
+    return (keys.new_empty(shape, dtype=torch.bfloat16), keys.new_empty(shape, dtype=torch.bfloat16))
+
+
+@torch.library.custom_op("wam_ffn::cache_attention", mutates_args=("work",))
+def _attend_op(q: torch.Tensor, heads: int, causal: bool, key_split: int, keys: torch.Tensor, values: torch.Tensor,
+               key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+               work: torch.Tensor) -> torch.Tensor:
+    cache = KVCache8._of(keys, values, key_scales, value_scales, block_table, lengths, work)
+    return cache._attend(q, heads, causal, key_split)
+
+
+@_attend_op.register_fake
+def _attend_fake(q, heads, causal, key_split, keys, values, key_scales, value_scales, block_table, lengths, work):
+    return q.new_empty(q.shape)
+
+
 class KVCache8:
     """Keys and values of ``batch`` sequences in e4m3 blocks of 64 tokens, head dim 128.
 
@@ -94,11 +145,15 @@ class KVCache8:
     def of(cls, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
            block_table: torch.Tensor, lengths: torch.Tensor) -> "KVCache8":
         """A cache over tensors that the caller holds (laid out as the class describes)."""
+        return cls._of(keys, values, key_scales, value_scales, block_table, lengths, None)
+
+    @classmethod
+    def _of(cls, keys, values, key_scales, value_scales, block_table, lengths, work):
         self = cls.__new__(cls)
-        self._hold(keys, values, key_scales, value_scales, block_table, lengths)
+        self._hold(keys, values, key_scales, value_scales, block_table, lengths, work)
         return self
 
-    def _hold(self, keys, values, key_scales, value_scales, block_table, lengths):
+    def _hold(self, keys, values, key_scales, value_scales, block_table, lengths, work=None):
         if keys.dim() != 4 or not keys.is_cuda:
             raise ValueError(f"keys must be a CUDA tensor [blocks, kv_heads, {BLOCK}, {HEAD_DIM}]")
         device, (pool, kv_heads) = keys.device, keys.shape[:2]
@@ -118,12 +173,11 @@ class KVCache8:
         self.block_table, self.lengths = block_table, lengths
         self.batch, self.width, self.kv_heads, self.device = batch, width, kv_heads, device
         self._needs: dict[tuple, int] = {}  # workspace of the attention, by its sizes
-        self._work = torch.zeros(batch + 1, dtype=torch.int32, device=device)  # tickets, status word
-        self._view = _lib.CacheView(
-            keys=keys.data_ptr(), values=values.data_ptr(), key_scales=key_scales.data_ptr(),
-            value_scales=value_scales.data_ptr(), block_table=block_table.data_ptr(), table_stride=width,
-            lengths=lengths.data_ptr(), tickets=self._work.data_ptr(), status=self._work.data_ptr() + 4 * batch,
-            blocks=pool, kv_heads=kv_heads, batch=batch, width=width)
+        self._work = torch.zeros(batch + 1, dtype=torch.int32, device=device) if work is None else work
+        self._view = _layout(keys, values, key_scales, value_scales, block_table, lengths, self._work)
+
+    def _tensors(self):
+        return (self.keys, self.values, self.key_scales, self.value_scales, self.block_table, self.lengths, self._work)
 
     @property
     def capacity(self) -> int:
@@ -148,6 +202,11 @@ class KVCache8:
         rounded to the new one.  A sequence whose rows do not fit (past capacity, ``at``
         beyond its length, a block id outside the pool) keeps what it had, and
         ``status`` reports it."""
+        if torch.compiler.is_compiling():
+            return _append_op(k, v, counts, at, *self._tensors())
+        self._append(k, v, counts, at)
+
+    def _append(self, k, v, counts, at):
         width = self.kv_heads * HEAD_DIM
         (k_view, k), (v_view, v) = (_rows(k, "k", self.batch, width, self.device),
                                     _rows(v, "v", self.batch, width, self.device))
@@ -163,6 +222,12 @@ class KVCache8:
         """Rows [start, start + count) of every sequence as bf16, k and v
         [batch, count, kv_heads * 128]; ``start`` a number or int32 [batch].
         Rows that a sequence does not hold are zeros."""
+        if torch.compiler.is_compiling():
+            tensor = isinstance(start, torch.Tensor)
+            return _read_op(count, start if tensor else None, 0 if tensor else start, *self._tensors())
+        return self._read(count, start)
+
+    def _read(self, count, start):
         tensor = isinstance(start, torch.Tensor)
         if count < 1 or (not tensor and not 0 <= start < 2 ** 31):
             raise ValueError(f"read of {count} rows from {start}")
@@ -182,6 +247,11 @@ class KVCache8:
         row that sees nothing is zeros.  NaN comes out where a row sees it: of a
         query or key in the whole of its heads, of a value in its dim.  key_split:
         CTAs of a cluster sharing a query tile's keys (0 = chosen; 1, 2, 4, 8)."""
+        if torch.compiler.is_compiling():
+            return _attend_op(q, heads, causal, key_split, *self._tensors())
+        return self._attend(q, heads, causal, key_split)
+
+    def _attend(self, q, heads, causal, key_split):
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"heads={heads} must be a multiple of the cache's {self.kv_heads}")
         view, q = _rows(q, "q", self.batch, heads * HEAD_DIM, self.device)

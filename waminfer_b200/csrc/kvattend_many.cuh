@@ -13,6 +13,11 @@
 //     shared memory in 8 bits (a ring of raw blocks there left room for three operand
 //     stages instead of five: 107 instead of 62 us for 32 rows over 16384, 24 heads).
 //
+// On a B200, 392 queries of 24 heads over 32768 rows take 213 us: 743 TFLOP/s, 45 % of
+// the measured bf16 GEMM burst; a step of both tiles 1.2 us, the chain of a tile's
+// products, row maximum and exponentials (P of step j must be read before S of
+// step j + 2 takes its columns; TMEM has no room for a third buffer).
+//
 //   warps 8-11, 12-15  softmax of tile 0 and 1, a query row a thread: Q to f16 in shared
 //                   memory once; per step the row maximum, P = 2^(x - m) in f16 over
 //                   S's own TMEM columns, O rescaled only when the maximum has grown by

@@ -12,6 +12,10 @@
 // would buy no precision, only up to one more binade above its smallest normal
 // value; in return x / 2^e and a change of scale are exact shifts, and
 // the attention folds the scales into its exponents.
+// Bound: HBM, 3 bytes an element to store and to read back.  2 x 8001 rows of 24
+// heads stored and read take 108 us on a B200, 84 % of its measured copy
+// bandwidth; 16 single tokens 6.1 us, latency (two launches).  Rows start on
+// their way before the block ids are checked: with the checks first 139 us.
 #pragma once
 
 #include "ptx.cuh"

@@ -12,7 +12,10 @@
 // in fp32, rounded to bf16 once (the reference rounds after the norm, after the
 // weight and after the rotation; one rounding is nearer to the formula).
 //
-// Bound: HBM, 4 bytes an element.  A lane holds 8 dims of a head in registers
+// Bound: HBM, 4 bytes an element: 2 x 8191 tokens of 32 + 8 heads take 53.7 us on a
+// B200, 98 % of its measured copy bandwidth, norm of each head (up to 8 heads a
+// group of lanes; 59 us with 4, 74 us with 2: fewer loads in flight, the table's
+// entries and addresses made for fewer heads).  One token takes 3 us: latency.  A lane holds 8 dims of a head in registers
 // (16 bytes in, 16 out) as two runs of 4, laid so that both members of every
 // pair are in the lane: the rotation needs no exchange.  A lane keeps its dims
 // for all the heads it visits, so its 4 table entries are read once.

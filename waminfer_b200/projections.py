@@ -15,8 +15,9 @@ them through the ``wam_ffn::prepared_ffn_linear_v1`` op.  A row count that was
 not prepared falls back to the module's own linear, as ``PreparedFFN`` does.
 
 The modulated norms around these projections are the library's
-``wam_ffn::modulated_norm`` (``waminfer_b200/norm.py``); the Q/K RMSNorm +
-RoPE and the attention kernels stay with the caller.
+``wam_ffn::modulated_norm`` (``waminfer_b200/norm.py``), the Q/K RMSNorm + RoPE
+is ``waminfer_b200/rope.py``, the attention ``waminfer_b200/attention.py`` and,
+over keys and values held in 8 bits, ``waminfer_b200/cache.py``.
 """
 
 from __future__ import annotations

@@ -20,84 +20,115 @@ import torch
 from waminfer_b200 import _lib
 
 
-def _side(x, weight, heads, name):
-    """Head dim, strides and the operand itself (a copy if the kernel cannot read its rows in place) of q or k."""
+def _check_side(x, weight, heads, name):
+    """Head dim of q or k after its checks."""
     if x.dim() != 3 or x.dtype != torch.bfloat16 or not x.is_cuda:
         raise ValueError(f"{name} must be a bf16 CUDA tensor [batch, rows, heads * head_dim]")
-    _, rows, width = x.shape
+    width = x.shape[2]
     if heads < 1 or width % heads:
         raise ValueError(f"{name} {tuple(x.shape)} does not hold {heads} heads")
-    dim, n = width // heads, weight.numel()
-    if weight.dtype != torch.bfloat16 or weight.dim() != 1 or (n != dim and n != width) or \
+    dim = width // heads
+    if weight.dtype != torch.bfloat16 or weight.dim() != 1 or weight.numel() not in (dim, width) or \
             not weight.is_contiguous() or weight.device != x.device:
         raise ValueError(f"{name}_weight must be a contiguous bf16 vector of {dim} (each head) or {width} "
                          f"(the row) on {x.device}")
+    return dim
+
+
+def _in_place(x):
+    """Whether the kernel can read the rows of q or k as they lie (but for the start's alignment)."""
     sb, sr, se = x.stride()
-    if se != 1 or sb % 8 or sr % 8 or x.data_ptr() % 16 or (sr < width and rows > 1):
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-        sb, sr, _ = x.stride()
-    return dim, _lib.RowsView(x.data_ptr(), sr, sb), x
+    return se == 1 and sb % 8 == 0 and sr % 8 == 0 and (sr >= x.shape[2] or x.shape[1] <= 1)
 
 
-def _vector(w):
-    return w if w.data_ptr() % 16 == 0 else w.clone()
-
-
-def _run(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved):
-    dim, q_view, q_held = _side(q, q_weight, heads, "q")
+def _checked(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved):
+    """The call's arguments without its pointers, after all checks of shapes, types and devices."""
+    dim = _check_side(q, q_weight, heads, "q")
     batch, rows, width = q.shape
-    device = q.device
     whole = q_weight.numel() != dim
-    k_view, k_at, k_out = _lib.RowsView(), None, None
     if k is not None:
         if k_weight is None:
             raise ValueError("k needs k_weight")
-        k_dim, k_view, k_held = _side(k, k_weight, kv_heads, "k")
-        if k_dim != dim or k.shape[:2] != q.shape[:2] or k.device != device:
+        if _check_side(k, k_weight, kv_heads, "k") != dim or k.shape[:2] != q.shape[:2] or k.device != q.device:
             raise ValueError(f"q {tuple(q.shape)} ({heads} heads) and k {tuple(k.shape)} ({kv_heads} heads) differ in "
                              "batch, rows, head dim or device")
         whole = whole or k_weight.numel() != dim
         if whole and (q_weight.numel() != width or k_weight.numel() != k.shape[2]):
             raise ValueError("q_weight and k_weight must both be for each head or both for the row")
-        k_weight = _vector(k_weight)
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-        k_at = k_out.data_ptr()
-    else:
-        kv_heads = 0
-    table = places = None
-    table_stride = table_rows = pairs = place_bytes = place_stride = 0
+    args = _lib.QkRopeArgs(batch=batch, rows=rows, heads=heads, kv_heads=0 if k is None else kv_heads, head_dim=dim,
+                           whole_row=whole, interleaved=interleaved, eps=eps)
     if rope is not None:
-        shape = rope.shape
-        if rope.dtype != torch.complex64 or rope.device != device or not (
-                len(shape) == 2 or (len(shape) == 3 and shape[1] == 1)) or rope.stride(-1) != 1:
-            raise ValueError(f"rope must be a complex64 table [positions, pairs] (or [positions, 1, pairs]) on {device}")
-        if rope.is_conj():
-            rope = rope.resolve_conj()
-        table, table_stride, table_rows, pairs = rope.data_ptr(), rope.stride(0), shape[0], shape[-1]
-        if table % 16 or table_stride % 2:
-            rope = rope.clone(memory_format=torch.contiguous_format)
-            table, table_stride = rope.data_ptr(), rope.stride(0)
+        if rope.dtype != torch.complex64 or rope.device != q.device or not (
+                rope.dim() == 2 or (rope.dim() == 3 and rope.shape[1] == 1)) or rope.stride(-1) != 1:
+            raise ValueError(f"rope must be a complex64 table [positions, pairs] (or [positions, 1, pairs]) on {q.device}")
+        args.table_stride, args.table_rows, args.pairs = rope.stride(0), rope.shape[0], rope.shape[-1]
         if positions is not None:
-            shape, kind = positions.shape, positions.dtype
-            if (kind != torch.int32 and kind != torch.int64) or positions.device != device or (
-                    shape != (batch, rows) and shape != (rows,)):
-                raise ValueError(f"positions must be int32 or int64, [{rows}] or [{batch}, {rows}], on {device}")
-            if rows > 1 and positions.stride(-1) != 1:
-                positions = positions.contiguous()
-            places, place_bytes = positions.data_ptr(), 4 if kind == torch.int32 else 8
-            place_stride = positions.stride(0) if len(shape) == 2 else 0
+            if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device or \
+                    tuple(positions.shape) not in ((rows,), (batch, rows)):
+                raise ValueError(f"positions must be int32 or int64, [{rows}] or [{batch}, {rows}], on {q.device}")
+            args.position_bytes = positions.element_size()
+            args.position_stride = positions.stride(0) if positions.dim() == 2 else 0
     elif positions is not None:
         raise ValueError("positions without a rope table")
+    plain = _in_place(q) and (k is None or _in_place(k)) and (rope is None or rope.stride(0) % 2 == 0) and (
+        positions is None or rows <= 1 or positions.stride(-1) == 1)
+    return bytes(args), plain, q.device.index
+
+
+# What _checked found for the shapes, strides and types of a call; a decode loop makes the same one over and over.
+_CHECKED: dict[tuple, tuple] = {}
+
+
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _aligned(t):
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _run(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved):
+    key = (_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(rope), _layout(positions), heads,
+           kv_heads, eps, interleaved)
+    found = _CHECKED.get(key)
+    if found is None:
+        if len(_CHECKED) >= 4096:
+            _CHECKED.clear()
+        found = _CHECKED[key] = _checked(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved)
+    raw, plain, device = found
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if q.numel() == 0:
-        return q_out, k_out
-    q_weight = _vector(q_weight)
-    args = _lib.QkRopeArgs(q_view, k_view, q_weight.data_ptr(), None if k is None else k_weight.data_ptr(), table,
-                           table_stride, places, place_stride, q_out.data_ptr(), k_at, place_bytes, table_rows, pairs,
-                           batch, rows, heads, kv_heads, dim, whole, interleaved, eps)
-    _lib.launch(_lib.lib().wamffn_qk_norm_rope, device.index, ctypes.byref(args))
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    if rope is not None and rope.is_conj():
+        rope = rope.resolve_conj()
+    if not plain:  # rows that the kernel cannot read as they lie: copies of them
+        if q.numel() == 0:
+            return q_out, k_out
+        q, k = q.contiguous(), None if k is None else k.contiguous()
+        rope = None if rope is None else rope.contiguous()
+        positions = None if positions is None else positions.contiguous()
+        args = _lib.QkRopeArgs.from_buffer_copy(
+            _checked(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved)[0])
+    else:
+        args = _lib.QkRopeArgs.from_buffer_copy(raw)
+        if not args.rows * args.batch:
+            return q_out, k_out
+    q, q_weight = _aligned(q), _aligned(q_weight)
+    sb, sr, _ = q.stride()
+    args.q = _lib.RowsView(q.data_ptr(), sr, sb)
+    args.q_weight, args.q_out = q_weight.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        k, k_weight = _aligned(k), _aligned(k_weight)
+        sb, sr, _ = k.stride()
+        args.k = _lib.RowsView(k.data_ptr(), sr, sb)
+        args.k_weight, args.k_out = k_weight.data_ptr(), k_out.data_ptr()
+    if rope is not None:
+        table = _aligned(rope)
+        if table is not rope:
+            args.table_stride = table.stride(0)
+        args.rope = table.data_ptr()
+        if positions is not None:
+            args.positions = positions.data_ptr()
+    _lib.launch(_lib.lib().wamffn_qk_norm_rope, device, ctypes.byref(args))
     return q_out, k_out
 
 
