@@ -1940,27 +1940,32 @@ size_t part_bytes(const KvAttnParams& p) {
 // on the device, so the table's width stands for them.
 struct KvAttnPlan {
   bool many;
-  int split, parts;
+  int split, parts, tile_rows;
   int64_t row_tiles;
 };
 
 KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, int most_parts) {
   const int64_t rows = int64_t(p.nq) * p.group;
-  KvAttnPlan plan{rows > kFewRows, key_split ? key_split : 1, 1, 1};
+  KvAttnPlan plan{rows > kFewRows, key_split ? key_split : 1, 1, kManyRows, 1};
   if (plan.many) {
-    // The least waves x (steps of a CTA + what a CTA costs besides, about four steps) + what parts cost, about six;
-    // clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
-    plan.row_tiles = (rows + kManyRows - 1) / kManyRows;
-    const int64_t ctas = plan.row_tiles * p.c.kv_heads * p.c.batch;
+    // The least waves x (steps of a CTA + what it costs besides) + what parts cost, in quarters of a step of 256 rows:
+    // a step of at most 128 rows (both tiles on the same rows) takes three, a CTA's start and end sixteen, the second
+    // kernel twenty-four.  Clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
     const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
     int64_t best = 0;
-    for (int s = 1; s <= 8; ++s) {
-      if (key_split ? s != key_split : 2 * s > std::max<int64_t>(steps, 2)) continue;
-      const int64_t at_once = s == 1 ? sm : many_clusters(s);
-      if (at_once < 1) continue;
-      for (int n = 1; n <= most_parts && (n == 1 || 4 * s * n <= steps); ++n) {
-        const int64_t cost = (ctas * n + at_once - 1) / at_once * ((steps + s * n - 1) / (s * n) + 4) + (n > 1 ? 6 : 0);
-        if (best == 0 || cost < best) best = cost, plan.split = s, plan.parts = n;
+    for (int tile_rows : {kManyRows, kManyRows / 2}) {
+      const int64_t tiles = (rows + tile_rows - 1) / tile_rows, ctas = tiles * p.c.kv_heads * p.c.batch;
+      const int step = rows <= kManyRows / 2 || tile_rows < kManyRows ? 3 : 4;
+      for (int s = 1; s <= 8; ++s) {
+        if (key_split ? s != key_split : 2 * s > std::max<int64_t>(steps, 2)) continue;
+        const int64_t at_once = s == 1 ? sm : many_clusters(s);
+        if (at_once < 1) continue;
+        for (int n = 1; n <= most_parts && (n == 1 || 4 * s * n <= steps); ++n) {
+          const int64_t cost =
+              (ctas * n + at_once - 1) / at_once * ((steps + s * n - 1) / (s * n) * step + 16) + (n > 1 ? 24 : 0);
+          if (best == 0 || cost < best)
+            best = cost, plan.split = s, plan.parts = n, plan.tile_rows = tile_rows, plan.row_tiles = tiles;
+        }
       }
     }
     return plan;
@@ -2108,6 +2113,7 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   const KvAttnPlan plan = plan_cache_attention(p, a->key_split, sm, most);
   p.split = plan.split;
   p.parts = plan.parts;
+  p.tile_rows = plan.tile_rows;
   const int64_t rows = int64_t(p.c.batch) * p.nq * p.heads;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + size_t(plan.parts) * rows * kCacheDim);

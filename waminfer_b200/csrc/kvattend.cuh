@@ -35,6 +35,7 @@ struct KvAttnParams {
   long long q_row, q_batch;  // strides, elements
   __nv_bfloat16* out;        // [batch, nq, heads 128]
   int nq, heads, group, causal, split;
+  int tile_rows;             // many rows: packed rows of a CTA, 256 or 128
   int parts;                 // of the keys, each with a cluster of its own
   float* part_o;             // parts > 1: unnormalised rows [parts, batch, nq, heads, 128]
   float2* part_ml;           // and their (maximum, normaliser) [parts, batch, nq, heads]

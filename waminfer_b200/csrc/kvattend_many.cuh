@@ -9,9 +9,9 @@
 //     the even steps in one and the odd steps in the other;
 //   - each tile has two S buffers: S of step j + 1 is there before P of step j is,
 //     so neither the warps nor the tensor cores wait for a step's whole chain;
-//   - the rows go from global memory to registers two steps ahead, never through
-//     shared memory in 8 bits (a ring of raw blocks there left room for three operand
-//     stages instead of five: 107 instead of 62 us for 32 rows over 16384, 24 heads).
+//   - blocks arrive by bulk copies, as they are held, two steps ahead of their
+//     conversion.  (Loads to registers instead are slower the further ahead they are:
+//     the fence between a conversion's stores and the products waits for them.)
 //
 // On a B200, 392 queries of 24 heads over 32768 rows take 213 us: 743 TFLOP/s, 45 % of
 // the measured bf16 GEMM burst; a step of both tiles 1.2 us, the chain of a tile's
@@ -22,9 +22,10 @@
 //                   memory once; per step the row maximum, P = 2^(x - m) in f16 over
 //                   S's own TMEM columns, O rescaled only when the maximum has grown by
 //                   more than 2^8 (P then stays below f16's range)
-//   warps 4-7       e4m3 -> f16, stored as 128-byte-swizzled operand tiles (K: K-major
+//   warps 4-7       e4m3 -> f16 through registers, stored as 128-byte-swizzled operand tiles (K: K-major
 //                   operand of Q K^T; V as it lies: MN-major operand of P V)
-//   warps 0, 1      one thread a tile issues S = Q K^T and O += P V; warps 2 and 3 are idle
+//   warps 0, 1      one thread a tile issues S = Q K^T and O += P V; warp 3 is idle
+//   warp 2          bulk copies of the blocks, 8 KB of K and of V, and their scales
 //
 // TMEM: S of tile x, step j at 128 x + 64 (j & 1), O of tile x at 256 + 128 x.
 // `split` CTAs of a cluster share a row tile's steps (of a part) and meet through
@@ -45,14 +46,17 @@ constexpr int kManySoftmaxWarps = 8, kManyConvWarps = 4;
 constexpr int kManyConvWarp0 = 4, kManySoftmaxWarp0 = 8;
 constexpr int kManyThreads = 16 * 32;
 // Registers a thread, by warpgroup: the launch gives every thread 128 (65536 / 512); the warpgroup of the issuing
-// threads hands over what the others take (64 + 144 + 2 * 152 = 4 * 128).
-constexpr int kManyLaunchRegs = 128, kManyMmaRegs = 64, kManyConvRegs = 144, kManySoftmaxRegs = 152;
+// threads hands over what the others take (80 + 112 + 2 * 160 = 4 * 128).
+constexpr int kManyLaunchRegs = 128, kManyMmaRegs = 80, kManyConvRegs = 112, kManySoftmaxRegs = 160;
 static_assert(kManyMmaRegs + kManyConvRegs + 2 * kManySoftmaxRegs <= 4 * kManyLaunchRegs, "register split");
 constexpr int kManyHalf = kManyStep * 64 * 2;   // 64 rows x 64 f16: half of an operand tile
 constexpr int kManyOperand = 2 * kManyHalf;     // 16 KB
-constexpr int kManyStages = 5;                  // of K, and of V
+constexpr int kManyStages = 5;                  // of K, and of V, in f16, with one tile's Q; one less with two
+constexpr int kManyRaw = 2;                     // blocks (K and V) as they are held, 16 KB each
 constexpr int kManyQuery = 2 * 128 * 64 * 2;    // Q of a tile: two halves of 128 rows x 64 f16
-constexpr int kManyData = 2 * kManyQuery + 2 * kManyStages * kManyOperand;
+constexpr int kManyOperands = kManyQuery + 2 * kManyStages * kManyOperand;  // Q and the stages
+static_assert(kManyQuery == 2 * kManyOperand, "a second Q takes a stage's place");
+constexpr int kManyData = kManyOperands + kManyRaw * 2 * kCacheTile;
 constexpr int kManyPitch = kCacheDim + 4;       // floats between rows of a partial result
 constexpr uint32_t kManyO = 256;  // TMEM column of tile 0's O
 
@@ -100,13 +104,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // Scales of a block for the softmax: x = S (qf kf) + ev, normaliser += sum P * back.
 struct ManyScale {
-  float kf, ev, back, pad;
+  float kf, ev, back, there;
 };
 
 struct ManyShared {
   uint64_t q_full, s_full[2][2], p_full[2][2];            // S, P: tile, buffer
   uint64_t o_step[2], o_last[2];                         // a step's, the last step's product into O is complete: tile
   uint64_t full[2][kManyStages], empty[2][kManyStages];  // operand tiles: K / V
+  uint64_t raw_full[kManyRaw], raw_empty[kManyRaw];
   ManyScale scale[8];                                    // of the steps in flight
   int nan_key[kCacheDim];
   int nan_any, abort_flag;
@@ -115,13 +120,11 @@ struct ManyShared {
 constexpr int kManySmem = 1024 + kManyData + int(sizeof(ManyShared));
 static_assert(kManySmem <= 232448, "227 KB a CTA");
 static_assert(kManyRows * (kManyPitch * 4 + 8) <= kManyData, "partial rows fit the operands' place");
-static_assert(kManyStages + 2 < 8, "a step's scales outlive its stage");
+static_assert(kManyStages + kManyRaw < 8, "a step's scales are kept until it is done");
 
 __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const KvAttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // Operand tile of K (w = 0) or V (w = 1), stage s.
-  auto operand = [&](int w, int s) { return smem + 2 * kManyQuery + (w * kManyStages + s) * kManyOperand; };
   ManyShared& sh = *reinterpret_cast<ManyShared*>(smem + kManyData);
   volatile int* abort = &sh.abort_flag;
 
@@ -130,10 +133,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   // The last row tile first: with a causal mask it has the most keys.
   const int shares = split * p.parts, share = int(blockIdx.x) % shares;  // of the keys: rank of the cluster in its part
   const int tile = int(gridDim.x) / shares - 1 - int(blockIdx.x) / shares, rank = share % split, part = share / split;
-  const int total_rows = p.nq * p.group, row0 = tile * kManyRows;
-  const int rows = min(kManyRows, total_rows - row0);
+  const int total_rows = p.nq * p.group, row0 = tile * p.tile_rows;
+  const int rows = min(p.tile_rows, total_rows - row0);
   const bool dual = rows <= 128;  // both tiles hold the same rows and take every second step
   const int stride = dual ? 2 : 1;
+  const int stages = dual ? kManyStages : kManyStages - 1;
+  // Q of tile x (dual: the same for both), operand tile of K (w = 0) or V (w = 1) in stage s, raw block r.
+  auto query = [&](int x) { return smem + (dual ? 0 : x) * kManyQuery; };
+  auto operand = [&](int w, int s) {
+    return smem + (dual ? 1 : 2) * kManyQuery + (w * stages + s) * kManyOperand;
+  };
+  auto raw_block = [&](int r) { return smem + kManyOperands + r * 2 * kCacheTile; };
 
   if (threadIdx.x == 0) {
     mbar_init(smem_addr(&sh.q_full), kManySoftmaxWarps);
@@ -148,6 +158,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         mbar_init(smem_addr(&sh.full[x][s]), kManyConvWarps);
         mbar_init(smem_addr(&sh.empty[x][s]), dual ? 1 : 2);  // tiles that read a step
       }
+    }
+    for (int r = 0; r < kManyRaw; ++r) {
+      mbar_init(smem_addr(&sh.raw_full[r]), 1);
+      mbar_init(smem_addr(&sh.raw_empty[r]), kManyConvWarps);
     }
     sh.abort_flag = 0;
     sh.nan_any = 0;
@@ -182,7 +196,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       constexpr uint32_t idesc_s = umma_idesc_f16(128, kManyStep);
       constexpr uint32_t idesc_o = umma_idesc_f16(128, kCacheDim) | (1u << 16);  // V MN-major
       const int x = warp;
-      const uint32_t ts = tmem + x * 128, to = tmem + kManyO + x * 128, qa = smem_addr(smem + x * kManyQuery);
+      const uint32_t ts = tmem + x * 128, to = tmem + kManyO + x * 128, qa = smem_addr(query(x));
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return wait_spin(smem_addr(bar), parity, abort, c.status, WAMFFN_DEV_TIMEOUT);
       };
@@ -200,8 +214,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       bool ok = wait(&sh.q_full, 0u) && wait(&sh.full[0][first_step], 0u);
       tc_fence_after();
       if (ok) issue_s(0, first_step);
-      int s = first_step, n = (first_step + stride) % kManyStages;  // stages of this tile's steps i and i + 1
-      uint32_t ph = 0, phn = first_step + stride >= kManyStages;    // and their phases
+      int s = first_step, n = first_step + stride;  // stages of this tile's steps i and i + 1
+      uint32_t ph = 0, phn = 0;                     // and their phases
       for (int i = 0, j = first_step; j < steps && ok; ++i, j += stride) {
         // S of the next step goes over P of the one before: that step's product must be complete (products of
         // different shapes are not ordered among themselves).
@@ -224,9 +238,63 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         umma_commit(smem_addr(&sh.empty[1][s]));
         s = n, ph = phn;
         n += stride;
-        if (n >= kManyStages) n -= kManyStages, phn ^= 1u;
+        if (n >= stages) n -= stages, phn ^= 1u;
       }
       umma_commit(smem_addr(&sh.o_last[x]));
+    }
+    if (warp == 2) {
+      // ---------------------------------------------------------- blocks and their scales
+      const int* table = c.table + b * c.table_stride;
+      auto id_of = [&](int i) { return i < steps ? table[first + i] : -1; };
+      int chunk = 0, id = id_of(lane), next_id = id_of(32 + lane);  // of steps 32 chunk + lane, and of the 32 after
+      float ks = 0.f, vs = 0.f;
+      auto load_scales = [&]() {
+        if (id < 0 || id >= c.blocks) {
+          id = -1;
+        } else {
+          const size_t at = size_t(id) * c.kv_heads + kh;
+          ks = c.key_scales[at];
+          vs = c.value_scales[at];
+        }
+      };
+      load_scales();
+      int r = 0, sent = 0, ok = 1;
+      uint32_t ph = 1u;
+      for (int j = 0; j < steps; ++j) {
+        if ((j >> 5) != chunk) {
+          chunk = j >> 5;
+          id = next_id;
+          load_scales();
+          next_id = id_of(32 * chunk + 32 + lane);
+        }
+        const int at = __shfl_sync(0xffffffffu, id, j & 31);
+        const float kj = __shfl_sync(0xffffffffu, ks, j & 31), vj = __shfl_sync(0xffffffffu, vs, j & 31);
+        if (lane == 0) {
+          const uint32_t bar = smem_addr(&sh.raw_full[r]), dst = smem_addr(raw_block(r));
+          if (j >= kManyRaw) ok = wait_spin(smem_addr(&sh.raw_empty[r]), ph, abort, c.status, WAMFFN_DEV_TIMEOUT);
+          if (ok) {
+            if (at >= 0) {
+              const int ev = scale_exp(vj);
+              sh.scale[j & 7] = ManyScale{exp2_int(scale_exp(kj)), float(ev), exp2_int(-ev), 1.f};
+              mbar_arrive_expect_tx(bar, 2 * kCacheTile);
+              const size_t from = (size_t(at) * c.kv_heads + kh) * kCacheTile;
+              bulk_load(dst, c.keys + from, kCacheTile, bar);
+              bulk_load(dst + kCacheTile, c.values + from, kCacheTile, bar);
+            } else {
+              sh.scale[j & 7] = ManyScale{1.f, -INFINITY, 0.f, 0.f};  // a block that is not there: nothing seen
+              if (c.status) atomicOr(c.status, WAMFFN_DEV_BAD_INDEX);
+              mbar_arrive_local(bar);
+            }
+            sent = j + 1;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (++r == kManyRaw) r = 0, ph ^= 1u;
+      }
+      if (lane == 0 && *abort)  // copies in flight land before the shared memory is given up
+        for (int j = max(0, sent - kManyRaw); j < sent; ++j)
+          wait_drain(smem_addr(&sh.raw_full[j % kManyRaw]), uint32_t(j / kManyRaw) & 1u);
     }
     __syncwarp();
     if (split > 1 || dual) {  // the softmax warps' two cluster barriers
@@ -236,74 +304,51 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   } else if (warp < kManySoftmaxWarp0) {
     // ------------------------------------------------------------ e4m3 -> f16
     set_registers<kManyConvRegs>();
-    // Thread: 16 bytes `chunk` (dims 16 chunk ..) of rows r0 + 16 i of the block.  Eight neighbouring lanes store
-    // four chunks of an even and of an odd row: eight different 16-byte columns of the swizzle.
+    // Thread: 16 bytes `chunk` (dims 16 chunk ..) of rows r0 + 16 i, 32 bytes of operand half chunk / 4.  Lanes of
+    // the upper dims store their second half first: eight neighbouring lanes then meet eight different 16-byte
+    // columns of the swizzle.
     const int tid = threadIdx.x - kManyConvWarp0 * 32;
-    const int c4 = tid & 3, half = (tid >> 3) & 1, r0 = ((tid >> 2) & 1) + 2 * (tid >> 4), chunk = 4 * half + c4;
-    const size_t in_tile = size_t(r0) * kCacheDim + chunk * 16;
-    const int* table = c.table + b * c.table_stride;
-    struct Raw {
-      uint4 k[4], v[4];
-      float ks, vs;  // scales; 0: no such block
-    };
-    auto id_of = [&](int j) { return j < steps ? table[first + j] : -1; };  // used a step later: nothing waits for it
-    auto load = [&](Raw& r, int id, bool wanted) {
-      if (id >= 0 && id < c.blocks) {
-        const size_t at = size_t(id) * c.kv_heads + kh;
-        const uint8_t *k = c.keys + at * kCacheTile + in_tile, *v = c.values + at * kCacheTile + in_tile;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          r.k[i] = *reinterpret_cast<const uint4*>(k + i * 16 * kCacheDim);
-          r.v[i] = *reinterpret_cast<const uint4*>(v + i * 16 * kCacheDim);
-        }
-        r.ks = c.key_scales[at];
-        r.vs = c.value_scales[at];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);
-        r.ks = r.vs = 0.f;
-        if (wanted && c.status && tid == 0) atomicOr(c.status, WAMFFN_DEV_BAD_INDEX);
-      }
-    };
+    const int chunk = tid & 7, r0 = tid >> 3, upper = chunk >> 2, column = 2 * (chunk & 3);
+    int s = 0, r = 0;                    // operand stage, raw block
+    uint32_t parity = 1u, raw_ph = 0u;   // of the stage's last use; of the block
     bool ok = true;
-    int s = 0;              // stage of the step
-    uint32_t parity = 1u;   // of the stage's last use
-    // Step j from its registers: both operand tiles into stage s.
-    auto convert = [&](Raw& r, int j) {
+    for (int j = 0; j < steps; ++j) {
       const int key0 = (first + j) * kManyStep;
-      if (j >= kManyStages) {  // the products of step j - kManyStages have read the stage
-        if (lane == 0)
+      if (lane == 0) {
+        ok = wait_spin(smem_addr(&sh.raw_full[r]), raw_ph, abort, c.status, WAMFFN_DEV_TIMEOUT);
+        if (ok && j >= stages)  // the products of step j - stages have read the stage
           ok = wait_spin(smem_addr(&sh.empty[0][s]), parity, abort, c.status, WAMFFN_DEV_TIMEOUT) &&
                wait_spin(smem_addr(&sh.empty[1][s]), parity, abort, c.status, WAMFFN_DEV_TIMEOUT);
-        ok = __shfl_sync(0xffffffffu, int(ok), 0);
-        if (!ok) return;
       }
-      if (tid == 0) {
-        ManyScale m{1.f, -INFINITY, 0.f, 0.f};  // a block that is not there: nothing seen
-        if (r.ks > 0.f) {
-          const int ev = scale_exp(r.vs);
-          m = ManyScale{exp2_int(scale_exp(r.ks)), float(ev), exp2_int(-ev), 0.f};
-        }
-        sh.scale[j & 7] = m;
-      }
+      ok = __shfl_sync(0xffffffffu, int(ok), 0);
+      if (!ok) break;
+      const bool there = sh.scale[j & 7].there != 0.f;
+      const uint32_t src = smem_addr(raw_block(r) + r0 * kCacheDim + chunk * 16);
+      uint4 raw[2][4];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          raw[w][i] = there ? lds128(src + w * kCacheTile + i * 16 * kCacheDim) : make_uint4(0, 0, 0, 0);
       if (key0 + kManyStep > least) {  // some row sees less than the whole step
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          r.v[i] = clean_chunk(r.v[i], key0 + r0 + 16 * i, length, least < most, 16 * chunk, sh.nan_key, &sh.nan_any);
+          raw[1][i] = clean_chunk(raw[1][i], key0 + r0 + 16 * i, length, least < most, 16 * chunk, sh.nan_key, &sh.nan_any);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(smem_addr(&sh.raw_empty[r]));
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        uint8_t* dst = operand(w, s) + half * kManyHalf;
+        uint8_t* dst = operand(w, s) + upper * kManyHalf;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint4 raw = w ? r.v[i] : r.k[i];
+          const uint4 u = raw[w][i];
           const int row = r0 + 16 * i;
-          *reinterpret_cast<uint4*>(dst + sw128_offset(row, 2 * c4)) =
-              make_uint4(e4m3x2_to_f16x2(raw.x), e4m3x2_hi_to_f16x2(raw.x), e4m3x2_to_f16x2(raw.y),
-                         e4m3x2_hi_to_f16x2(raw.y));
-          *reinterpret_cast<uint4*>(dst + sw128_offset(row, 2 * c4 + 1)) =
-              make_uint4(e4m3x2_to_f16x2(raw.z), e4m3x2_hi_to_f16x2(raw.z), e4m3x2_to_f16x2(raw.w),
-                         e4m3x2_hi_to_f16x2(raw.w));
+          const uint32_t a = upper ? u.z : u.x, z = upper ? u.w : u.y, a2 = upper ? u.x : u.z, z2 = upper ? u.y : u.w;
+          *reinterpret_cast<uint4*>(dst + sw128_offset(row, column + upper)) =
+              make_uint4(e4m3x2_to_f16x2(a), e4m3x2_hi_to_f16x2(a), e4m3x2_to_f16x2(z), e4m3x2_hi_to_f16x2(z));
+          *reinterpret_cast<uint4*>(dst + sw128_offset(row, column + 1 - upper)) =
+              make_uint4(e4m3x2_to_f16x2(a2), e4m3x2_hi_to_f16x2(a2), e4m3x2_to_f16x2(z2), e4m3x2_hi_to_f16x2(z2));
         }
       }
       fence_proxy_async();
@@ -312,22 +357,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         mbar_arrive_local(smem_addr(&sh.full[0][s]));
         mbar_arrive_local(smem_addr(&sh.full[1][s]));
       }
-      if (++s == kManyStages) s = 0, parity ^= 1u;
-    };
-    // Two steps in registers, block ids a step further ahead.
-    Raw even, odd;
-    load(even, id_of(0), steps > 0);
-    load(odd, id_of(1), steps > 1);
-    int ahead0 = id_of(2), ahead1 = id_of(3);
-    for (int j = 0; j < steps && ok; j += 2) {
-      convert(even, j);
-      load(even, ahead0, j + 2 < steps);
-      ahead0 = id_of(j + 4);
-      if (j + 1 < steps && ok) {
-        convert(odd, j + 1);
-        load(odd, ahead1, j + 3 < steps);
-        ahead1 = id_of(j + 5);
-      }
+      if (++s == stages) s = 0, parity ^= 1u;
+      if (++r == kManyRaw) r = 0, raw_ph ^= 1u;
     }
     __syncwarp();
     if (split > 1 || dual) {
@@ -365,7 +396,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = f16x2_pack(bf2_lo(u[4 * i + e]) * inv, bf2_hi(u[4 * i + e]) * inv);
-        *reinterpret_cast<uint4*>(smem + x * kManyQuery + (i >> 3) * (kManyQuery / 2) + sw128_offset(r & 127, i & 7)) =
+        *reinterpret_cast<uint4*>(query(x) + (i >> 3) * (kManyQuery / 2) + sw128_offset(r & 127, i & 7)) =
             make_uint4(w[0], w[1], w[2], w[3]);
       }
       fence_proxy_async();
