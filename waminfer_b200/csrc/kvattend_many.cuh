@@ -34,6 +34,8 @@
 // share the instruction cache.
 #pragma once
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "kvattend.cuh"
 
@@ -551,24 +553,51 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       cluster_sync();
       // Rank order; rank k takes rows k, k + split, ...
       const int pieces = ((rows - rank + split - 1) / split) * (kCacheDim / 4);
-      for (int i = r; i < pieces; i += kManySoftmaxWarps * 32) {
-        const int pr = rank + (i >> 5) * split, d = (i & 31) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float top = -INFINITY, sum = 0.f;
-        for (int k = 0; k < split * stride; ++k) {  // CTA, and tile where both hold the row
-          const int from = dual ? k >> 1 : k, at = pr + (dual ? 128 * (k & 1) : 0);
-          const float2 ml = ld_cluster2(map_to_cta(smem_addr(&held_ml[at]), from));
-          const float4 u = ld_cluster4(map_to_cta(smem_addr(held + at * kManyPitch + d), from));
-          const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
-          const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
-          v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
-          v.z = v.z * fo + u.z * fn, v.w = v.w * fo + u.w * fn;
-          sum = sum * fo + ml.y * fn;
-          top = next;
+      auto merge = [&](auto batch) {  // pieces of a thread whose loads are in flight together
+        constexpr int kBatch = decltype(batch)::value;
+        for (int i0 = r; i0 < pieces; i0 += kBatch * kManySoftmaxWarps * 32) {
+          float4 v[kBatch];
+          float top[kBatch], sum[kBatch];
+  #pragma unroll
+          for (int q = 0; q < kBatch; ++q) {
+            v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+            top[q] = -INFINITY;
+            sum[q] = 0.f;
+          }
+          for (int k = 0; k < split * stride; ++k) {  // CTA, and tile where both hold the row
+            const int from = dual ? k >> 1 : k;
+            float2 ml[kBatch];
+            float4 u[kBatch];
+  #pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+              const int i = min(i0 + q * kManySoftmaxWarps * 32, pieces - 1);
+              const int at = rank + (i >> 5) * split + (dual ? 128 * (k & 1) : 0), d = (i & 31) * 4;
+              ml[q] = ld_cluster2(map_to_cta(smem_addr(&held_ml[at]), from));
+              u[q] = ld_cluster4(map_to_cta(smem_addr(held + at * kManyPitch + d), from));
+            }
+  #pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+              const float next = fmaxf(top[q], ml[q].x), safe = next == -INFINITY ? 0.f : next;
+              const float fo = ex2_approx(top[q] - safe), fn = ex2_approx(ml[q].x - safe);
+              v[q].x = v[q].x * fo + u[q].x * fn, v[q].y = v[q].y * fo + u[q].y * fn;
+              v[q].z = v[q].z * fo + u[q].z * fn, v[q].w = v[q].w * fo + u[q].w * fn;
+              sum[q] = sum[q] * fo + ml[q].y * fn;
+              top[q] = next;
+            }
+          }
+  #pragma unroll
+          for (int q = 0; q < kBatch; ++q) {
+            const int i = i0 + q * kManySoftmaxWarps * 32;
+            const int prow = row0 + rank + (i >> 5) * split, ptoken = prow / p.group;
+            const int phead = kh * p.group + prow - ptoken * p.group;
+            if (i < pieces && !*abort) kv_emit(p, part, b, ptoken, phead, (i & 31) * 4, v[q], top[q], sum[q]);
+          }
         }
-        const int prow = row0 + pr, ptoken = prow / p.group, phead = kh * p.group + prow - ptoken * p.group;
-        if (!*abort) kv_emit(p, part, b, ptoken, phead, d, v, top, sum);
-      }
+      };
+      if (pieces > kManySoftmaxWarps * 32)
+        merge(std::integral_constant<int, 4>{});
+      else
+        merge(std::integral_constant<int, 1>{});
       __syncwarp();
       cluster_sync();  // no CTA leaves while a peer reads its shared memory
     }
