@@ -112,7 +112,7 @@ struct ManyScale {
 struct ManyShared {
   uint64_t q_full, s_full[2][2], p_full[2][2];            // S, P: tile, buffer
   uint64_t o_step[2], o_last[2];                         // a step's, the last step's product into O is complete: tile
-  uint64_t full[2][kManyStages], empty[2][kManyStages];  // operand tiles: K / V
+  uint64_t full[kManyStages], empty[kManyStages];        // K and V of a step in f16
   uint64_t raw_full[kManyRaw], raw_empty[kManyRaw];
   ManyScale scale[8];                                    // of the steps in flight
   int nan_key[kCacheDim];
@@ -156,10 +156,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         mbar_init(smem_addr(&sh.s_full[x][i]), 1);
         mbar_init(smem_addr(&sh.p_full[x][i]), 4);
       }
-      for (int s = 0; s < kManyStages; ++s) {
-        mbar_init(smem_addr(&sh.full[x][s]), kManyConvWarps);
-        mbar_init(smem_addr(&sh.empty[x][s]), dual ? 1 : 2);  // tiles that read a step
-      }
+    }
+    for (int s = 0; s < kManyStages; ++s) {
+      mbar_init(smem_addr(&sh.full[s]), kManyConvWarps);
+      mbar_init(smem_addr(&sh.empty[s]), dual ? 1 : 2);  // tiles that read a step
     }
     for (int r = 0; r < kManyRaw; ++r) {
       mbar_init(smem_addr(&sh.raw_full[r]), 1);
@@ -210,24 +210,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           umma_bf16(ts + i * 64, umma_desc_sw128(qa + (k >> 2) * (kManyQuery / 2)) + 2 * (k & 3),
                     umma_desc_sw128(ka + (k >> 2) * kManyHalf) + 2 * (k & 3), idesc_s, k ? 1u : 0u);
         umma_commit(smem_addr(&sh.s_full[x][i]));
-        umma_commit(smem_addr(&sh.empty[0][s]));
       };
       const int first_step = dual ? x : 0;
-      bool ok = wait(&sh.q_full, 0u) && wait(&sh.full[0][first_step], 0u);
+      bool ok = wait(&sh.q_full, 0u) && wait(&sh.full[first_step], 0u);
       tc_fence_after();
       if (ok) issue_s(0, first_step);
       int s = first_step, n = first_step + stride;  // stages of this tile's steps i and i + 1
-      uint32_t ph = 0, phn = 0;                     // and their phases
+      uint32_t phn = 0;                             // phase of n
       for (int i = 0, j = first_step; j < steps && ok; ++i, j += stride) {
         // S of the next step goes over P of the one before: that step's product must be complete (products of
         // different shapes are not ordered among themselves).
         if (j + stride < steps) {
-          ok = wait(&sh.full[0][n], phn) && (i == 0 || wait(&sh.o_step[x], uint32_t(i - 1) & 1u));
+          ok = wait(&sh.full[n], phn) && (i == 0 || wait(&sh.o_step[x], uint32_t(i - 1) & 1u));
           if (!ok) break;
           tc_fence_after();
           issue_s((i + 1) & 1, n);
         }
-        ok = wait(&sh.full[1][s], ph) && wait(&sh.p_full[x][i & 1], uint32_t(i >> 1) & 1u);
+        ok = wait(&sh.p_full[x][i & 1], uint32_t(i >> 1) & 1u);
         if (!ok) break;
         tc_fence_after();
         const uint32_t va = smem_addr(operand(1, s));
@@ -237,8 +236,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
                       umma_desc_sw128_mn(va + uint32_t(k) * 2 * kVGroupBytes, kManyHalf, kVGroupBytes), idesc_o,
                       (i | k) ? 1u : 0u);
         umma_commit(smem_addr(&sh.o_step[x]));
-        umma_commit(smem_addr(&sh.empty[1][s]));
-        s = n, ph = phn;
+        umma_commit(smem_addr(&sh.empty[s]));
+        s = n;
         n += stride;
         if (n >= stages) n -= stages, phn ^= 1u;
       }
@@ -319,8 +318,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       if (lane == 0) {
         ok = wait_spin(smem_addr(&sh.raw_full[r]), raw_ph, abort, c.status, WAMFFN_DEV_TIMEOUT);
         if (ok && j >= stages)  // the products of step j - stages have read the stage
-          ok = wait_spin(smem_addr(&sh.empty[0][s]), parity, abort, c.status, WAMFFN_DEV_TIMEOUT) &&
-               wait_spin(smem_addr(&sh.empty[1][s]), parity, abort, c.status, WAMFFN_DEV_TIMEOUT);
+          ok = wait_spin(smem_addr(&sh.empty[s]), parity, abort, c.status, WAMFFN_DEV_TIMEOUT);
       }
       ok = __shfl_sync(0xffffffffu, int(ok), 0);
       if (!ok) break;
@@ -355,10 +353,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_local(smem_addr(&sh.full[0][s]));
-        mbar_arrive_local(smem_addr(&sh.full[1][s]));
-      }
+      if (lane == 0) mbar_arrive_local(smem_addr(&sh.full[s]));
       if (++s == stages) s = 0, parity ^= 1u;
       if (++r == kManyRaw) r = 0, raw_ph ^= 1u;
     }
