@@ -435,6 +435,51 @@ def test_refusals(cuda_device):
     assert not cache.attend(good, 2).any()  # an empty cache
 
 
+def test_views_and_another_stream(cuda_device):
+    """Queries as a chunk of a packed projection, in another row order, unaligned; on a side stream."""
+    cache, g = make(cuda_device, 2, 2, 2, [300, 77], spread=1)
+    packed = rows(g, 2, 21, 3 * 512)
+    q = packed[..., 512:1024]
+    expect = cache.attend(q.contiguous(), 4, causal=True)
+    assert torch.equal(cache.attend(q, 4, causal=True), expect)
+    assert torch.equal(cache.attend(q.transpose(0, 1).contiguous().transpose(0, 1), 4, causal=True), expect)
+    odd = torch.empty(q.numel() + 1, dtype=torch.bfloat16, device=cuda_device)[1:].view(q.shape)
+    odd.copy_(q)
+    assert torch.equal(cache.attend(odd, 4, causal=True), expect)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = cache.attend(q, 4, causal=True)
+        read = cache.read(10)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(there, expect) and torch.equal(read[0], cache.read(10)[0])
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Blocks at the end of a pool of 2.6 GB of keys, and query rows past 2^31 elements."""
+    from waminfer_b200.cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    k, v = rows(g, 1, 200, 8 * DIM), rows(g, 1, 200, 8 * DIM)
+    small, large = KVCache8(1, 256, 8, cuda_device), KVCache8(1, 256, 8, cuda_device, blocks=40000)
+    large.block_table[0] = torch.tensor([39999, 32768, 39000, 1], dtype=torch.int32)
+    for cache in (small, large):
+        cache.append(k[:, :130], v[:, :130])
+        cache.append(k[:, 130:], v[:, 130:])
+    for a, b in zip(small.read(200), large.read(200)):
+        assert torch.equal(a, b)
+    for nq in (1, 30, 300):
+        q = rows(g, 1, nq, 16 * DIM)
+        assert torch.equal(small.attend(q, 16), large.attend(q, 16))
+    assert large.status() == 0
+    del large
+    one = KVCache8(1, 64, 1, cuda_device)
+    one.append(k[:, :40, :DIM], v[:, :40, :DIM])
+    q = rows(g, 1, 530000, 32 * DIM)
+    tail = one.attend(q, 32)[:, -5:].clone()
+    close(tail, attention(Model(one), q[:, -5:], 32, False), 40)
+
+
 # ------------------------------------------------------------- together
 def test_a_decode_run(cuda_device):
     """A prompt, then tokens one by one: norm and rotation, store, attention; eagerly and from one captured step."""

@@ -171,6 +171,19 @@ def test_captured_and_on_another_stream(cuda_device):
     assert torch.equal(held[0], expect[0]) and torch.equal(held[1], expect[1])
 
 
+@pytest.mark.parametrize("whole", [False, True])
+def test_offsets_past_32_bits(cuda_device, whole):
+    from waminfer_b200.rope import qk_norm_rope
+
+    q, k, qw, kw, g = case(cuda_device, 9, 1, 1, 32, 4, 64, whole)
+    q = torch.randn(1, 1 << 20, 2048, device=cuda_device, generator=g, dtype=torch.bfloat16)  # 2^31 elements
+    q = torch.cat((q, q[:, :700]), 1)
+    freqs = table(1 << 21, 32, cuda_device)
+    out, _ = qk_norm_rope(q, None, qw, None, freqs, None, 32)
+    at = torch.arange(q.shape[1] - 700, q.shape[1], device=cuda_device)
+    check(out[:, -700:], reference(q[:, -700:], qw, freqs[at][None].to(torch.complex128), 32, 1e-6, True))
+
+
 def test_the_reference_on_the_same_rows(cuda_device):
     """The reference's rounding points (bf16 after the norm and after the weight) move a value by up to
     three half steps: 3 * 2^-8 of it and of its pair."""
