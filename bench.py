@@ -277,10 +277,14 @@ def _cpu_sample(geo, requests: int, seconds: float, threads: int) -> dict:
 
 def cpu_baseline(geo, min_seconds: float = 10.0):
     """The reference's CPU FFN path timed on all host cores over whole requests
-    (at least `min_seconds` of work after one untimed warm-up request)."""
+    (at least `min_seconds` of work after one untimed warm-up request); the
+    reason in words where the reference is not installed."""
     threads = os.cpu_count() or 1
     torch.set_num_threads(threads)
-    ref = CpuReference(geo)
+    try:
+        ref = CpuReference(geo)
+    except FileNotFoundError as exc:
+        return {"unavailable": str(exc)}
     ref.request()
     requests, seconds = ref.time_requests(min_seconds)
     return _cpu_sample(geo, requests, seconds, threads)
