@@ -147,6 +147,19 @@ def test_queries_alone_views_and_positions_outside(cuda_device):
     assert qk_norm_rope(q[:, :0], None, qw, None, freqs, None, 4)[0].shape == (2, 0, 512)
 
 
+def test_conjugated_table_of_wider_rows(cuda_device):
+    """A lazily conjugated slice: turned the other way, by the slice's own entries."""
+    from waminfer_b200.rope import qk_norm_rope
+
+    q, k, qw, kw, _ = case(cuda_device, 11, 2, 30, 4, 4, 128, True)
+    wide = table(30, 96, cuda_device)
+    back = wide.conj()[:, :64]
+    assert back.is_conj()
+    turn = wide[:, :64].conj().resolve_conj()[None].to(torch.complex128).expand(2, 30, 64)
+    for rope in (back, back[:, None]):
+        check(qk_norm_rope(q, None, qw, None, rope, None, 4)[0], reference(q, qw, turn, 4, 1e-6, True))
+
+
 def test_captured_and_on_another_stream(cuda_device):
     from waminfer_b200.rope import qk_norm_rope
 

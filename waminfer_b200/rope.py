@@ -88,6 +88,8 @@ def _aligned(t):
 
 
 def _run(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved):
+    if rope is not None and rope.is_conj():  # before anything looks at its strides: the copy may have others
+        rope = rope.resolve_conj()
     key = (_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(rope), _layout(positions), heads,
            kv_heads, eps, interleaved)
     found = _CHECKED.get(key)
@@ -98,8 +100,6 @@ def _run(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interl
     raw, plain, device = found
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
-    if rope is not None and rope.is_conj():
-        rope = rope.resolve_conj()
     if not plain:  # rows that the kernel cannot read as they lie: copies of them
         if q.numel() == 0:
             return q_out, k_out
