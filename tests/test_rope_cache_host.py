@@ -119,3 +119,11 @@ def test_python_refuses_what_it_cannot_run():
     with pytest.raises(ValueError, match="CUDA"):
         KVCache8.of(blocks, blocks, torch.ones(2, 1), torch.ones(2, 1), torch.zeros(1, 2, dtype=torch.int32),
                     torch.zeros(1, dtype=torch.int32))
+
+
+def test_keys_without_their_weight():
+    from waminfer_b200.rope import qk_norm_rope
+
+    q, w = torch.zeros(1, 4, 256, dtype=torch.bfloat16), torch.ones(128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        qk_norm_rope(q, q, w, None, None, None, 2, 2)
