@@ -455,6 +455,19 @@ def test_views_and_another_stream(cuda_device):
     assert torch.equal(there, expect) and torch.equal(read[0], cache.read(10)[0])
 
 
+def test_status_of_calls_on_another_stream(cuda_device):
+    from waminfer_b200.cache import KVCache8
+
+    cache = KVCache8(1, 64, 1, cuda_device)
+    x = torch.ones(1, 65, DIM, dtype=torch.bfloat16, device=cuda_device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # about 50 ms
+        cache.append(x, x)  # does not fit
+    assert cache.status() == 2 and cache.status() == 0 and cache.lengths.tolist() == [0]
+
+
 def test_offsets_past_32_bits(cuda_device):
     """Blocks at the end of a pool of 2.6 GB of keys, and query rows past 2^31 elements."""
     from waminfer_b200.cache import KVCache8

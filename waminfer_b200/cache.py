@@ -281,6 +281,7 @@ class KVCache8:
 
     def status(self, clear: bool = True) -> int:
         """Device status word (timeout / bad-index bits); synchronises the device."""
+        torch.cuda.synchronize(self.device)  # the calls may be on other streams than the copy below
         value = int(self._work[self.batch])
         if clear and value:
             self._work[self.batch:].zero_()
