@@ -609,16 +609,17 @@ typedef struct wamffn_cache_view {
 } wamffn_cache_view;
 
 /* Stores rows k, v [batch, rows, kv_heads * 128] bf16 (strides in elements,
- * multiples of 8) at row at[b] of sequence b (at NULL: lengths[b]) and sets
- * lengths[b] = at[b] + counts[b]; counts NULL: rows; rows past counts[b] (a
- * padded batch) are not stored.  at[b] < lengths[b] replaces the rows from there
- * on.  Scale of a block and head: 2^e, the least e >= -60 with
- * |x| <= 448 * 2^e for its finite values; a block that holds rows in front of
- * the new ones keeps at least the scale it has, and when that grows those rows
- * are turned over to it.  Values are rounded to the nearest e4m3 (even on
- * ties); infinities become +-448 * 2^e, NaN stays.  A sequence whose rows do not
- * fit (at[b] outside [0, lengths[b]], past width * 64 rows, a block id outside
- * [0, blocks)) is left unchanged and sets WAMFFN_DEV_BAD_INDEX. */
+ * multiples of 8; that of a single row or batch is not used) at row at[b] of
+ * sequence b (at NULL: lengths[b]) and sets lengths[b] = at[b] + counts[b];
+ * counts NULL: rows; rows past counts[b] (a padded batch) are not stored.
+ * at[b] < lengths[b] replaces the rows from there on.  Scale of a block and
+ * head: 2^e, the least e >= -60 with |x| <= 448 * 2^e for its finite values; a
+ * block that holds rows in front of the new ones keeps at least the scale it
+ * has, and when that grows those rows are turned over to it.  Values are rounded
+ * to the nearest e4m3 (even on ties); infinities become +-448 * 2^e, NaN stays.
+ * A sequence whose rows do not fit (at[b] outside [0, lengths[b]], past
+ * width * 64 rows, a block id outside [0, blocks)) is left unchanged and sets
+ * WAMFFN_DEV_BAD_INDEX. */
 typedef struct wamffn_cache_append_args {
   wamffn_cache_view cache;
   wamffn_rows_view k, v;

@@ -160,6 +160,23 @@ def test_conjugated_table_of_wider_rows(cuda_device):
         check(qk_norm_rope(q, None, qw, None, rope, None, 4)[0], reference(q, qw, turn, 4, 1e-6, True))
 
 
+def test_a_single_batch_row_or_table_row_of_any_stride(cuda_device):
+    from waminfer_b200.rope import qk_norm_rope
+
+    q, _, qw, _, _ = case(cuda_device, 12, 1, 30, 4, 4, 128, True)
+    freqs = table(30, 64, cuda_device)
+    held = torch.zeros(1, 30 * 512 + 5, dtype=torch.bfloat16, device=cuda_device)
+    held[:, :30 * 512] = q.reshape(1, -1)
+    expect = qk_norm_rope(q, None, qw, None, freqs, None, 4)[0]
+    view = held[:, :30 * 512].view(1, 30, 512)
+    assert view.stride(0) % 8 and torch.equal(qk_norm_rope(view, None, qw, None, freqs, None, 4)[0], expect)
+    odd = torch.zeros(1, 1, 513, dtype=torch.bfloat16, device=cuda_device)
+    odd[..., :512] = q[:, :1]
+    one = torch.zeros(1, 65, dtype=torch.complex64, device=cuda_device)
+    one[:, :64] = freqs[:1]
+    assert torch.equal(qk_norm_rope(odd[..., :512], None, qw, None, one[:, :64], None, 4)[0], expect[:, :1])
+
+
 def test_captured_and_on_another_stream(cuda_device):
     from waminfer_b200.rope import qk_norm_rope
 

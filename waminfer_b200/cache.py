@@ -41,7 +41,7 @@ def _rows(t: torch.Tensor, name: str, batch: int, width: int,
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the 8-bit cache has no backward pass: run it with gradients disabled")
     sb, sr, se = t.stride()
-    if se != 1 or sb % 8 or sr % 8 or t.data_ptr() % 16 or (sr < width and rows > 1):
+    if se != 1 or (count > 1 and sb % 8) or (rows > 1 and (sr % 8 or sr < width)) or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

@@ -1775,11 +1775,13 @@ int wamffn_current_frame_attention(void* stream_, const wamffn_current_frame_arg
 // ================================================= norm + rotation, 8-bit cache
 namespace {
 
-// A [batch, rows, width] bf16 operand read row by row (any batch stride).
+// A [batch, rows, width] bf16 operand read row by row (any batch stride).  The stride of a single row or batch is
+// never used.
 int check_rows_view(const wamffn_rows_view& v, int64_t width, int rows, int batch, const char* name) {
   if (!v.data) return fail(WAMFFN_ERR_INVALID, "%s is null", name);
   if (!aligned16(v.data)) return fail(WAMFFN_ERR_INVALID, "%s must be 16-byte aligned", name);
-  if ((rows > 1 && v.row_stride < width) || v.row_stride % 8 || v.batch_stride < 0 || v.batch_stride % 8)
+  if ((rows > 1 && (v.row_stride < width || v.row_stride % 8)) ||
+      (batch > 1 && (v.batch_stride < 0 || v.batch_stride % 8)))
     return fail(WAMFFN_ERR_INVALID, "%s strides (%lld, %lld): multiples of 8 elements, rows >= %lld apart", name,
                 (long long)v.batch_stride, (long long)v.row_stride, (long long)width);
   return WAMFFN_OK;
@@ -2008,7 +2010,8 @@ int wamffn_qk_norm_rope(void* stream, const wamffn_qk_rope_args* a) {
   if (a->rope) {
     if (a->pairs < 4 || a->pairs % 4 || a->pairs > d / 2)
       return fail(WAMFFN_ERR_INVALID, "pairs=%d: a multiple of 4 up to %d", a->pairs, d / 2);
-    if (a->table_rows < 1 || (a->table_rows > 1 && a->table_stride < a->pairs) || a->table_stride % 2 || !aligned16(a->rope))
+    if (a->table_rows < 1 || (a->table_rows > 1 && (a->table_stride < a->pairs || a->table_stride % 2)) ||
+        !aligned16(a->rope))
       return fail(WAMFFN_ERR_INVALID, "rope table: %d rows, stride %lld (even, >= pairs), 16-byte aligned",
                   a->table_rows, (long long)a->table_stride);
     if (a->positions) {

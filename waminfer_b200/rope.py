@@ -38,7 +38,7 @@ def _check_side(x, weight, heads, name):
 def _in_place(x):
     """Whether the kernel can read the rows of q or k as they lie (but for the start's alignment)."""
     sb, sr, se = x.stride()
-    return se == 1 and sb % 8 == 0 and sr % 8 == 0 and (sr >= x.shape[2] or x.shape[1] <= 1)
+    return se == 1 and (sb % 8 == 0 or x.shape[0] <= 1) and (x.shape[1] <= 1 or (sr % 8 == 0 and sr >= x.shape[2]))
 
 
 def _checked(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved):
