@@ -372,6 +372,20 @@ def test_attend_nan_stays_where_it_is_seen(cuda_device, nq, heads, kv_heads):
         close(cache.attend(q, heads, causal=causal), attention(Model(cache), q, heads, causal), 200)
 
 
+@pytest.mark.parametrize("nq", [40, 200])
+def test_attend_shares_without_keys(cuda_device, nq):
+    """A cluster's CTAs that get no keys hand over nothing, whatever the queries hold: NaN queries stay in their rows."""
+    cache, g = make(cuda_device, 6, 3, 2, [0, 64, 130], capacity=1024)
+    q = rows(g, 3, nq, 4 * DIM)
+    q[:, ::3, :DIM] = float("nan")
+    for _ in range(5):
+        for split in (0, 2, 8):
+            out = cache.attend(q, 4, key_split=split)
+            nan = out.view(3, nq, 4, DIM).isnan()
+            assert not out[0].any() and nan[1:, ::3, 0].all()
+            assert int(nan.sum()) == 2 * len(range(0, nq, 3)) * DIM
+
+
 def test_attend_bad_blocks_and_lengths(cuda_device):
     """Block ids outside the pool are left out and reported; a length past the table is cut to it."""
     cache, g = make(cuda_device, 1, 2, 2, [190, 190], spread=1)

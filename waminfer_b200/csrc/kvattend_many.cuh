@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         if (n >= stages) n -= stages, phn ^= 1u;
       }
       umma_commit(smem_addr(&sh.o_last[x]));
+      if (!ok) wait_drain(smem_addr(&sh.o_last[x]), 0u);  // no product reads memory that is given up
     }
     if (warp == 2) {
       // ---------------------------------------------------------- blocks and their scales
@@ -482,11 +483,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       }
     }
     if (ok) {
-      // Both tiles: the operands' place is reused below.
-      if (lane == 0)
+      // Both tiles: the operands' place is reused below, by a CTA without steps too (every warp's Q is written then).
+      if (lane == 0) {
+        ok = wait_spin(smem_addr(&sh.q_full), 0u, abort, c.status, WAMFFN_DEV_TIMEOUT);
         for (int y = 0; y < 2; ++y)
           if ((dual ? y : 0) < steps)
             ok = ok && wait_spin(smem_addr(&sh.o_last[y]), 0u, abort, c.status, WAMFFN_DEV_TIMEOUT);
+      }
       ok = __shfl_sync(0xffffffffu, int(ok), 0);
       tc_fence_after();
     }
@@ -555,7 +558,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         for (int i0 = r; i0 < pieces; i0 += kBatch * kManySoftmaxWarps * 32) {
           float4 v[kBatch];
           float top[kBatch], sum[kBatch];
-  #pragma unroll
+#pragma unroll
           for (int q = 0; q < kBatch; ++q) {
             v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
             top[q] = -INFINITY;
@@ -565,14 +568,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
             const int from = dual ? k >> 1 : k;
             float2 ml[kBatch];
             float4 u[kBatch];
-  #pragma unroll
+#pragma unroll
             for (int q = 0; q < kBatch; ++q) {
               const int i = min(i0 + q * kManySoftmaxWarps * 32, pieces - 1);
               const int at = rank + (i >> 5) * split + (dual ? 128 * (k & 1) : 0), d = (i & 31) * 4;
               ml[q] = ld_cluster2(map_to_cta(smem_addr(&held_ml[at]), from));
               u[q] = ld_cluster4(map_to_cta(smem_addr(held + at * kManyPitch + d), from));
             }
-  #pragma unroll
+#pragma unroll
             for (int q = 0; q < kBatch; ++q) {
               const float next = fmaxf(top[q], ml[q].x), safe = next == -INFINITY ? 0.f : next;
               const float fo = ex2_approx(top[q] - safe), fn = ex2_approx(ml[q].x - safe);
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
               top[q] = next;
             }
           }
-  #pragma unroll
+#pragma unroll
           for (int q = 0; q < kBatch; ++q) {
             const int i = i0 + q * kManySoftmaxWarps * 32;
             const int prow = row0 + rank + (i >> 5) * split, ptoken = prow / p.group;
