@@ -168,7 +168,7 @@ def test_a_single_batch_row_or_table_row_of_any_stride(cuda_device):
     held = torch.zeros(1, 30 * 512 + 5, dtype=torch.bfloat16, device=cuda_device)
     held[:, :30 * 512] = q.reshape(1, -1)
     expect = qk_norm_rope(q, None, qw, None, freqs, None, 4)[0]
-    view = held[:, :30 * 512].view(1, 30, 512)
+    view = held.as_strided((1, 30, 512), (held.shape[1], 512, 1))
     assert view.stride(0) % 8 and torch.equal(qk_norm_rope(view, None, qw, None, freqs, None, 4)[0], expect)
     odd = torch.zeros(1, 1, 513, dtype=torch.bfloat16, device=cuda_device)
     odd[..., :512] = q[:, :1]
