@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           wait_drain(smem_addr(&sh.raw_full[j % kManyRaw]), uint32_t(j / kManyRaw) & 1u);
     }
     __syncwarp();
-    if (split > 1 || dual) {  // the softmax warps' two cluster barriers
+    if (split > 1) {  // the softmax warps' two cluster barriers
       cluster_sync();
       cluster_sync();
     }
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       if (++r == kManyRaw) r = 0, raw_ph ^= 1u;
     }
     __syncwarp();
-    if (split > 1 || dual) {
+    if (split > 1) {
       cluster_sync();
       cluster_sync();
     }
@@ -507,95 +507,133 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         for (int i = 0; i < 32; ++i)
           if (sh.nan_key[q * 32 + i] < seen) v[i] = 0x7fffffffu;
     };
-    if (split == 1 && !dual) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
-      __nv_bfloat16* dst = p.out + ((size_t(b) * p.nq + token) * p.heads + head) * kCacheDim;
-      if (ok) {
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t v[32];
-          load_o(q, v);
-          if (live && p.parts > 1) {
+    float* held = reinterpret_cast<float*>(smem);  // rows of O; every product has read the operands that lay there
+    float2* held_ml = reinterpret_cast<float2*>(held + kManyRows * kManyPitch);
+    auto place = [&](int at, int d) { return reinterpret_cast<float4*>(held + at * kManyPitch + d); };
+    auto emit = [&](int q, const uint32_t (&v)[32], float inv) {  // 32 dims of a row that is complete in this CTA
+      if (p.parts > 1) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              kv_emit(p, part, b, token, head, q * 32 + i,
-                      make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]),
-                                  __uint_as_float(v[i + 3])), m, l);
-          } else if (live) {
+        for (int i = 0; i < 32; i += 4)
+          kv_emit(p, part, b, token, head, q * 32 + i,
+                  make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]),
+                              __uint_as_float(v[i + 3])), m, l);
+      } else {
+        __nv_bfloat16* dst = p.out + ((size_t(b) * p.nq + token) * p.heads + head) * kCacheDim + q * 32;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              float o[8];
+        for (int i = 0; i < 32; i += 8) {
+          float o[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(v[i + e]) * inv;
-              *reinterpret_cast<uint4*>(dst + q * 32 + i) =
-                  make_uint4(bf2_pack(o[0], o[1]), bf2_pack(o[2], o[3]), bf2_pack(o[4], o[5]), bf2_pack(o[6], o[7]));
-            }
-          }
+          for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(v[i + e]) * inv;
+          *reinterpret_cast<uint4*>(dst + i) =
+              make_uint4(bf2_pack(o[0], o[1]), bf2_pack(o[2], o[3]), bf2_pack(o[4], o[5]), bf2_pack(o[6], o[7]));
         }
       }
-    } else {
-      // This CTA's partial rows (unnormalised O, maximum, normaliser) to shared memory; every product has read it.
-      float* held = reinterpret_cast<float*>(smem);
-      float2* held_ml = reinterpret_cast<float2*>(held + kManyRows * kManyPitch);
-      if (live) {
-        held_ml[r] = make_float2(m, l);
+    };
+    float f = 1.f;
+    if (dual) {
+      // The two tiles' shares of a row: each hands half of the dims to the other and adds what it gets to its half.
+      held_ml[r] = make_float2(m, l);
+      __syncwarp();
+      named_sync(1, kManySoftmaxWarps * 32);
+      const float2 e0 = held_ml[rr], e1 = held_ml[rr + 128];
+      const float top = fmaxf(e0.x, e1.x), safe = top == -INFINITY ? 0.f : top;
+      const float f0 = ex2_approx(e0.x - safe), f1 = ex2_approx(e1.x - safe);
+      f = x ? f1 : f0;
+      m = top;
+      l = e0.y * f0 + e1.y * f1;
+#pragma unroll 1
+      for (int q = x ? 0 : 2, n = 0; n < 2; ++n, ++q) {
+        uint32_t v[32];
+        load_o(q, v);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *place(rr, q * 32 + i) = make_float4(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f,
+                                               __uint_as_float(v[i + 2]) * f, __uint_as_float(v[i + 3]) * f);
       }
+      __syncwarp();
+      named_sync(1, kManySoftmaxWarps * 32);
+    }
+    if (dual) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int q = x ? 2 : 0, n = 0; n < 2; ++n, ++q) {
+        uint32_t v[32];
+        load_o(q, v);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 o = *place(rr, q * 32 + i);
+          v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), f, o.x));
+          v[i + 1] = __float_as_uint(fmaf(__uint_as_float(v[i + 1]), f, o.y));
+          v[i + 2] = __float_as_uint(fmaf(__uint_as_float(v[i + 2]), f, o.z));
+          v[i + 3] = __float_as_uint(fmaf(__uint_as_float(v[i + 3]), f, o.w));
+          if (split > 1) *reinterpret_cast<uint4*>(place(rr, q * 32 + i)) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+        if (split == 1 && live && ok) emit(q, v, inv);
+      }
+      if (split > 1 && x == 0) held_ml[rr] = make_float2(m, l);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
+      if (split > 1) held_ml[r] = make_float2(m, l);
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {
         uint32_t v[32];
         load_o(q, v);
-        if (live)
+        if (split == 1) {
+          if (live && ok) emit(q, v, inv);
+        } else {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(held + r * kManyPitch + q * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            *reinterpret_cast<uint4*>(place(r, q * 32 + i)) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
       }
+    }
+    if (split > 1) {
+      // The cluster's shares of the rows, in rank order; rank k takes rows k, k + split, ...
       __syncwarp();
       cluster_sync();
-      // Rank order; rank k takes rows k, k + split, ...
       const int pieces = ((rows - rank + split - 1) / split) * (kCacheDim / 4);
-      auto merge = [&](auto batch) {  // pieces of a thread whose loads are in flight together
-        constexpr int kBatch = decltype(batch)::value;
+      auto merge = [&](auto batch) {  // pieces of a thread whose eight loads are in flight together
+        constexpr int kBatch = decltype(batch)::value, kShares = 8 / kBatch;
         for (int i0 = r; i0 < pieces; i0 += kBatch * kManySoftmaxWarps * 32) {
-          float4 v[kBatch];
-          float top[kBatch], sum[kBatch];
+          float4 u[kBatch][kShares];
+          float2 ml[kBatch][kShares];
 #pragma unroll
-          for (int q = 0; q < kBatch; ++q) {
-            v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            top[q] = -INFINITY;
-            sum[q] = 0.f;
-          }
-          for (int k = 0; k < split * stride; ++k) {  // CTA, and tile where both hold the row
-            const int from = dual ? k >> 1 : k;
-            float2 ml[kBatch];
-            float4 u[kBatch];
+          for (int n = 0; n < kBatch; ++n) {
+            const int i = i0 + n * kManySoftmaxWarps * 32, at = rank + (i >> 5) * split;
+            const uint32_t ml_at = smem_addr(&held_ml[at]), o_at = smem_addr(place(at, (i & 31) * 4));
 #pragma unroll
-            for (int q = 0; q < kBatch; ++q) {
-              const int i = min(i0 + q * kManySoftmaxWarps * 32, pieces - 1);
-              const int at = rank + (i >> 5) * split + (dual ? 128 * (k & 1) : 0), d = (i & 31) * 4;
-              ml[q] = ld_cluster2(map_to_cta(smem_addr(&held_ml[at]), from));
-              u[q] = ld_cluster4(map_to_cta(smem_addr(held + at * kManyPitch + d), from));
-            }
-#pragma unroll
-            for (int q = 0; q < kBatch; ++q) {
-              const float next = fmaxf(top[q], ml[q].x), safe = next == -INFINITY ? 0.f : next;
-              const float fo = ex2_approx(top[q] - safe), fn = ex2_approx(ml[q].x - safe);
-              v[q].x = v[q].x * fo + u[q].x * fn, v[q].y = v[q].y * fo + u[q].y * fn;
-              v[q].z = v[q].z * fo + u[q].z * fn, v[q].w = v[q].w * fo + u[q].w * fn;
-              sum[q] = sum[q] * fo + ml[q].y * fn;
-              top[q] = next;
+            for (int k = 0; k < kShares; ++k) {
+              ml[n][k] = make_float2(-INFINITY, 0.f);
+              u[n][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (k < split && i < pieces) {
+                ml[n][k] = ld_cluster2(map_to_cta(ml_at, k));
+                u[n][k] = ld_cluster4(map_to_cta(o_at, k));
+              }
             }
           }
 #pragma unroll
-          for (int q = 0; q < kBatch; ++q) {
-            const int i = i0 + q * kManySoftmaxWarps * 32;
-            const int prow = row0 + rank + (i >> 5) * split, ptoken = prow / p.group;
-            const int phead = kh * p.group + prow - ptoken * p.group;
-            if (i < pieces && !*abort) kv_emit(p, part, b, ptoken, phead, (i & 31) * 4, v[q], top[q], sum[q]);
+          for (int n = 0; n < kBatch; ++n) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kShares; ++k) top = fmaxf(top, ml[n][k].x);
+            const float safe = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < kShares; ++k) {
+              const float fk = ex2_approx(ml[n][k].x - safe);
+              v.x += u[n][k].x * fk, v.y += u[n][k].y * fk, v.z += u[n][k].z * fk, v.w += u[n][k].w * fk;
+              sum += ml[n][k].y * fk;
+            }
+            const int i = i0 + n * kManySoftmaxWarps * 32, prow = row0 + rank + (i >> 5) * split;
+            const int ptoken = prow / p.group, phead = kh * p.group + prow - ptoken * p.group;
+            if (i < pieces && !*abort) kv_emit(p, part, b, ptoken, phead, (i & 31) * 4, v, top, sum);
           }
         }
       };
-      if (pieces > kManySoftmaxWarps * 32)
+      if (split == 2)
         merge(std::integral_constant<int, 4>{});
+      else if (split <= 4)
+        merge(std::integral_constant<int, 2>{});
       else
         merge(std::integral_constant<int, 1>{});
       __syncwarp();
