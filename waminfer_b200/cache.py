@@ -260,13 +260,13 @@ class KVCache8:
         if rows == 0:
             return out
         args = _lib.CacheAttentionArgs(self._view, view, out.data_ptr(), None, 0, rows, heads, causal, key_split)
-        held = self._parts(args, rows, heads, key_split)  # kept until the launch, then the stream's
+        held = self._parts(args, rows, heads, bool(causal), key_split)  # kept until the launch, then the stream's
         _lib.launch(_lib.lib().wamffn_cache_attention, self.device.index, ctypes.byref(args))
         return out
 
-    def _parts(self, args, rows: int, heads: int, key_split: int) -> torch.Tensor | None:
+    def _parts(self, args, rows: int, heads: int, causal: bool, key_split: int) -> torch.Tensor | None:
         """Gives the call its workspace; few query rows over a long cache ask for one."""
-        key = (rows, heads, key_split)
+        key = (rows, heads, causal, key_split)
         size = self._needs.get(key)
         if size is None:
             need = ctypes.c_size_t()

@@ -1950,21 +1950,31 @@ KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, in
   const int64_t rows = int64_t(p.nq) * p.group;
   KvAttnPlan plan{rows > kFewRows, key_split ? key_split : 1, 1, kManyRows, 1};
   if (plan.many) {
-    // The least waves x (steps of a CTA + what it costs besides) + what parts cost, in quarters of a step of 256 rows:
-    // a step of at most 128 rows (both tiles on the same rows) takes three, a CTA's start and end sixteen, the second
-    // kernel twenty-four.  Clusters of more CTAs leave more SMs without one (three: 45 clusters, 135 of 148 SMs).
+    // The least estimate, in units of 0.1 us: waves x (steps of a CTA + its start and end) + the second kernel.
+    // Measured on a B200: a step takes 1.2 us, with both tiles on the same rows (at most 128) 0.77 us; start and end
+    // 4.3 us; in a cluster 2.6 us more (its CTAs start and end together), 5 us with 256 rows to hand over; parts
+    // cost 2.5 us and 0.2 us each, and write and read fp32 rows at about 4 TB/s.  Clusters of more CTAs also leave
+    // more SMs without one (three: 45 clusters, 135 of 148 SMs).  With a causal mask the CTAs differ and fill the
+    // waves' gaps: their mean, and half of one at the end (16384 rows over 4096: 194 us; counted in whole waves,
+    // which takes clusters of two, 246 us).
     const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
+    const int64_t mean = p.causal ? std::max<int64_t>(1, steps - p.nq / (2 * kManyStep)) : steps;
     int64_t best = 0;
     for (int tile_rows : {kManyRows, kManyRows / 2}) {
       const int64_t tiles = (rows + tile_rows - 1) / tile_rows, ctas = tiles * p.c.kv_heads * p.c.batch;
-      const int step = rows <= kManyRows / 2 || tile_rows < kManyRows ? 3 : 4;
+      const bool dual = rows <= kManyRows / 2 || tile_rows < kManyRows;
       for (int s = 1; s <= 8; ++s) {
         if (key_split ? s != key_split : 2 * s > std::max<int64_t>(steps, 2)) continue;
         const int64_t at_once = s == 1 ? sm : many_clusters(s);
         if (at_once < 1) continue;
         for (int n = 1; n <= most_parts && (n == 1 || 4 * s * n <= steps); ++n) {
-          const int64_t cost =
-              (ctas * n + at_once - 1) / at_once * ((steps + s * n - 1) / (s * n) * step + 16) + (n > 1 ? 24 : 0);
+          auto cta = [&](int64_t all) {  // time of a CTA
+            return (all + s * n - 1) / (s * n) * (dual ? 77 : 120) / 10 + 43 + (s == 1 ? 0 : dual ? 26 : 50);
+          };
+          int64_t cost = (ctas * n + at_once - 1) / at_once * cta(steps);
+          if (p.causal && ctas * n > at_once)
+            cost = std::max(cta(steps), ctas * n * cta(mean) / at_once + cta(mean) / 2);
+          if (n > 1) cost += 25 + n * int64_t(2 + 2 * part_bytes(p) / 400000);
           if (best == 0 || cost < best)
             best = cost, plan.split = s, plan.parts = n, plan.tile_rows = tile_rows, plan.row_tiles = tiles;
         }
