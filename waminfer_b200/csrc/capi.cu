@@ -1955,8 +1955,8 @@ KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, in
     // 4.3 us; in a cluster 2.6 us more (its CTAs start and end together), 5 us with 256 rows to hand over; parts
     // cost 2.5 us and 0.2 us each, and write and read fp32 rows at about 4 TB/s.  Clusters of more CTAs also leave
     // more SMs without one (three: 45 clusters, 135 of 148 SMs).  With a causal mask the CTAs differ and fill the
-    // waves' gaps: their mean, and half of one at the end (16384 rows over 4096: 194 us; counted in whole waves,
-    // which takes clusters of two, 246 us).
+    // waves' gaps: their mean, and half of one at the end (16384 rows over 4096, head by head: 194 us; counted in
+    // whole waves, which takes clusters of two, 246 us).
     const int64_t steps = (int64_t(p.c.width) * kCacheBlock + kManyStep - 1) / kManyStep;
     const int64_t mean = p.causal ? std::max<int64_t>(1, steps - p.nq / (2 * kManyStep)) : steps;
     int64_t best = 0;

@@ -15,7 +15,7 @@
 //
 // On a B200, 512 queries of 37 heads over 16384 rows (every SM busy) run at 875 TFLOP/s,
 // 53 % of the measured bf16 GEMM burst, the tensor pipe 45 % and the exponentials'
-// 46 % of the cycles; 392 queries of 24 heads over 32768 rows take 214 us.  A step of
+// 46 % of the cycles; 392 queries of 24 heads over 32768 rows take 215 us.  A step of
 // both tiles takes 1.2 us: the chain of a tile's products, row maximum and exponentials
 // (P of step j must be read before S of step j + 2 takes its columns; TMEM has no
 // room for a third buffer).
@@ -133,10 +133,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   volatile int* abort = &sh.abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = p.split, kh = blockIdx.y, b = blockIdx.z;
-  // The last row tile first: with a causal mask it has the most keys.
+  const int split = p.split;
   const int shares = split * p.parts, share = int(blockIdx.x) % shares;  // of the keys: rank of the cluster in its part
-  const int tile = int(gridDim.x) / shares - 1 - int(blockIdx.x) / shares, rank = share % split, part = share / split;
+  const int rank = share % split, part = share / split;
+  // In the order of launch: with a causal mask the last row tile, which has the most keys, of every head, then the one
+  // before, so that the short ones even out the end (16384 rows over 4096: 167 us; 194 us head by head); without one
+  // head by head, whose CTAs then read the same blocks (392 queries over 32768 rows: 215 us; 216 us tile by tile).
+  const int tiles = int(gridDim.x) / shares, unit = int(blockIdx.y) * tiles + int(blockIdx.x) / shares;
+  const int b = blockIdx.z, kh = p.causal ? unit % int(gridDim.y) : int(blockIdx.y);
+  const int tile = tiles - 1 - (p.causal ? unit / int(gridDim.y) : int(blockIdx.x) / shares);
   const int total_rows = p.nq * p.group, row0 = tile * p.tile_rows;
   const int rows = min(p.tile_rows, total_rows - row0);
   const bool dual = rows <= 128;  // both tiles hold the same rows and take every second step
