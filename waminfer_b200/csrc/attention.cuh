@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (lane == 0)
         ok = wait_spin(smem_addr(q_full), 0u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT) &&
              wait_spin(smem_addr(&k_full[0]), 0u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = warp_verdict(ok);
     }
     if (ok) {
       tc_fence_after();
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           ok = wait_spin(smem_addr(&k_full[(j + 1) & 1]), uint32_t((j + 1) >> 1) & 1u, abort_flag, p.status,
                          WAMFFN_DEV_TIMEOUT) &&
                wait_spin(smem_addr(s_free), uint32_t(j) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = warp_verdict(ok);
         if (!ok) break;
         tc_fence_after();
         issue_s(j + 1);
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (lane == 0)
         ok = wait_spin(smem_addr(&v_full[j & 1]), uint32_t(j >> 1) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT) &&
              wait_spin(smem_addr(p_full), uint32_t(j) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = warp_verdict(ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t st = smem_addr(kv_s + (j & 1) * 4 * kAttnTile);
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int j = 0; j < nblocks; ++j) {
       if (lane == 0 && ok)
         ok = wait_spin(smem_addr(s_full), uint32_t(j) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = warp_verdict(ok);
       float sc[64];
       float bmax = -INFINITY;
       const AttnKeyBlock kb = block_of(jb + j);
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (j > 0) {
         if (lane == 0)
           ok = wait_spin(smem_addr(o_done), uint32_t(j - 1) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = warp_verdict(ok);
         if (!ok) continue;
         tc_fence_after();
 #pragma unroll
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     if (ok && nblocks > 0) {
       if (lane == 0)
         ok = wait_spin(smem_addr(o_done), uint32_t(nblocks - 1) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = warp_verdict(ok);
     }
     if (ok && rec && threadIdx.x == 0) rec[4] = globaltimer_ns();
     // O of this CTA (zero when it ran no key block: TMEM then holds nothing).
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       int got = 1;
       if (lane == 0) got = wait_spin(smem_addr(xch_full), 0u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-      got = __shfl_sync(0xffffffffu, got, 0);
+      got = warp_verdict(got);
       cluster_arrive();  // this CTA's incoming slots have landed
       if (rec && threadIdx.x == 0) rec[7] = globaltimer_ns();
       if (ok && got) {

@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // One lane polls; the verdict is broadcast so the warp stays converged.
       int ok = 1;
       if (lane == 0) ok = wait_bounded(smem_addr(&empty[s]), ph ^ 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (!warp_verdict(ok)) break;
       if (elect_one()) {
         const uint32_t local_full = smem_addr(&full[s]);
         // The leader's barrier counts both CTAs' bytes; the peer only adds its copies.
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           kb = beg1;
           if (lane == 0)
             ok = wait_bounded(smem_addr(tmem_empty), 0u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-          if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+          if (!warp_verdict(ok)) break;
           tc_fence_after();
         }
         const bool first_k = kb == (piece == 0 ? beg0 : beg1);
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             WAMFFN_DEV_TIMEOUT) &&
                wait_bounded(smem_addr(&full_b[sb]), uint32_t(i / p.b_stages) & 1u, abort_flag, p.status,
                             WAMFFN_DEV_TIMEOUT);
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        if (!warp_verdict(ok)) break;
         tc_fence_after();
         if (i == 0 && rec && lane == 0) rec[2] = globaltimer_ns();
         const uint64_t adesc = umma_desc_sw128(a0 + uint32_t(sa * a_bytes));
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     int ok = 0;
     if (lane == 0)
       ok = wait_bounded(smem_addr(&tmem_full[0]), 0u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT) && !*abort_flag;
-    ok = __shfl_sync(0xffffffffu, ok, 0);
+    ok = warp_verdict(ok);
     tc_fence_after();
     if (ok)
       sk_dump(tmem_base + (uint32_t(q * 32) << 16), my_slot + q * 32 + lane, (warp - kEpiWarp0) >> 2, 2, tokens);
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0)
       ok = wait_bounded(smem_addr(&tmem_full[npieces - 1]), 0u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT) &&
            !*abort_flag;
-    ok = __shfl_sync(0xffffffffu, ok, 0);
+    ok = warp_verdict(ok);
     tc_fence_after();
     unsigned long long* rec =
         (warp == kEpiWarp0 && lane == 0 && *trace_slot != 0xffffffffu) ? g_trace + size_t(*trace_slot) * kTraceWords
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = warp_verdict(ok);
     }
     if (kSK && ok && !owner) {
       // A CTA whose only piece is a helper piece: all 12 warps dump it.

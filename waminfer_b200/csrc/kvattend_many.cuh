@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
             sent = j + 1;
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = warp_verdict(ok);
         if (!ok) break;
         if (++r == kManyRaw) r = 0, ph ^= 1u;
       }
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         if (ok && j >= stages)  // the products of step j - stages have read the stage
           ok = wait_spin(smem_addr(&sh.empty[s]), parity, abort, c.status, WAMFFN_DEV_TIMEOUT);
       }
-      ok = __shfl_sync(0xffffffffu, int(ok), 0);
+      ok = warp_verdict(ok);
       if (!ok) break;
       const bool there = sh.scale[j & 7].there != 0.f;
       const uint32_t src = smem_addr(raw_block(r) + r0 * kCacheDim + chunk * 16);
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         const uint32_t ts = tmem + x * 128 + (n & 1) * 64 + lanes;
         if (lane == 0)
           ok = wait_spin(smem_addr(&sh.s_full[x][n & 1]), uint32_t(n >> 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
-        ok = __shfl_sync(0xffffffffu, int(ok), 0);
+        ok = warp_verdict(ok);
         if (!ok) break;
         tc_fence_after();
         uint32_t v[2][32];
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         if (__any_sync(0xffffffffu, grown) && n > 0) {
           if (lane == 0)
             ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(n - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
-          ok = __shfl_sync(0xffffffffu, int(ok), 0);
+          ok = warp_verdict(ok);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           if ((dual ? y : 0) < steps)
             ok = ok && wait_spin(smem_addr(&sh.o_last[y]), 0u, abort, c.status, WAMFFN_DEV_TIMEOUT);
       }
-      ok = __shfl_sync(0xffffffffu, int(ok), 0);
+      ok = warp_verdict(ok);
       tc_fence_after();
     }
     // 32 dims of this row's O; a NaN that was cleaned out of a value this row sees comes back.

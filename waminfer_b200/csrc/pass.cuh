@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kPassThreads, 1) stack_pass_kernel(const __gri
             go = pass_wait(p, p.bars + 3 * l + kind, nctas, abort_flag);
             if (unsigned long long* rec = pass_trace(p, l, 1 + kind)) rec[6] = globaltimer_ns();
           }
-          if (!__shfl_sync(0xffffffffu, go, 0)) {
+          if (!warp_verdict(go)) {
             ok = false;
             break;
           }
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kPassThreads, 1) stack_pass_kernel(const __gri
             const uint32_t ph = (n / uint32_t(stages)) & 1u;
             int w_ok = 1;
             if (lane == 0) w_ok = wait_bounded(smem_addr(&empty[s]), ph ^ 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-            if (!__shfl_sync(0xffffffffu, w_ok, 0)) {
+            if (!warp_verdict(w_ok)) {
               ok = false;
               break;
             }
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kPassThreads, 1) stack_pass_kernel(const __gri
               int w_ok = 1;
               if (lane == 0)
                 w_ok = wait_bounded(smem_addr(tmem_empty), (item - 1) & 1u, abort_flag, p.status, WAMFFN_DEV_TIMEOUT);
-              if (!__shfl_sync(0xffffffffu, w_ok, 0)) {
+              if (!warp_verdict(w_ok)) {
                 ok = false;
                 break;
               }
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(kPassThreads, 1) stack_pass_kernel(const __gri
                                     WAMFFN_DEV_TIMEOUT) &&
                        wait_bounded(smem_addr(&full_b[sb]), (nb / uint32_t(p.b_stages)) & 1u, abort_flag, p.status,
                                     WAMFFN_DEV_TIMEOUT);
-              if (!__shfl_sync(0xffffffffu, w_ok, 0)) {
+              if (!warp_verdict(w_ok)) {
                 ok = false;
                 break;
               }

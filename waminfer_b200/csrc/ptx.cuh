@@ -142,6 +142,14 @@ __device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
+// What lane 0 found by its wait, for the whole warp.  A shuffle orders no memory: the warp barrier behind it makes
+// what lane 0's wait made visible (bytes of a copy, stores of other warps) visible to the other lanes too.
+__device__ __forceinline__ int warp_verdict(int found) {
+  found = __shfl_sync(0xffffffffu, found, 0);
+  __syncwarp();
+  return found;
+}
+
 // Same wait without the abort shortcut, used to drain in-flight copies.
 __device__ __forceinline__ bool wait_drain(uint32_t bar, uint32_t parity) {
   const long long t0 = clock64();
