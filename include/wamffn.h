@@ -674,6 +674,24 @@ typedef struct wamffn_cache_attention_args {
 int wamffn_cache_attention_workspace(const wamffn_cache_attention_args* args, size_t* bytes);
 int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* args);
 
+/* How the call would share out its work with these arguments, its workspace
+ * among them: row_tiles tiles of up to tile_rows packed rows (query x head of a
+ * key head), each with `parts` clusters of key_split CTAs; tensor_cores: on
+ * tcgen05 (more than 16 packed rows), else on mma.sync.  sm_count and clusters
+ * are given: the device's SMs and, at [s], how many clusters of s CTAs it holds
+ * at once (nothing is asked of a GPU then); sm_count 0: the current device. */
+typedef struct wamffn_cache_plan {
+  int sm_count;
+  int clusters[9];
+  int tensor_cores;
+  int key_split;
+  int parts;
+  int tile_rows;
+  int64_t row_tiles;
+} wamffn_cache_plan;
+
+int wamffn_cache_attention_plan(const wamffn_cache_attention_args* args, wamffn_cache_plan* plan);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,7 @@ EXPORTED_SYMBOLS = (
     "wamffn_cache_read",
     "wamffn_cache_attention",
     "wamffn_cache_attention_workspace",
+    "wamffn_cache_attention_plan",
     "wamffn_rgb_mandatory",
     "wamffn_select_tokens",
     "wamffn_pack_weight",
@@ -221,6 +222,14 @@ class CacheAttentionArgs(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("nq", ctypes.c_int), ("heads", ctypes.c_int), ("causal", ctypes.c_int), ("key_split", ctypes.c_int)]
 
 
+class CachePlan(ctypes.Structure):
+    """Mirror of ``wamffn_cache_plan``."""
+
+    _fields_ = [("sm_count", ctypes.c_int), ("clusters", ctypes.c_int * 9),
+                *[(name, ctypes.c_int) for name in ("tensor_cores", "key_split", "parts", "tile_rows")],
+                ("row_tiles", ctypes.c_int64)]
+
+
 class BlockArgs(ctypes.Structure):
     """Mirror of ``wamffn_block_args``."""
 
@@ -344,6 +353,7 @@ def _declare(lib):
     lib.wamffn_cache_read.argtypes = [vp, ctypes.POINTER(CacheReadArgs)]
     lib.wamffn_cache_attention.argtypes = [vp, ctypes.POINTER(CacheAttentionArgs)]
     lib.wamffn_cache_attention_workspace.argtypes = [ctypes.POINTER(CacheAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
+    lib.wamffn_cache_attention_plan.argtypes = [ctypes.POINTER(CacheAttentionArgs), ctypes.POINTER(CachePlan)]
     lib.wamffn_rgb_mandatory.argtypes = [vp, vp, vp, i, i, i, i, vp]
     lib.wamffn_select_tokens.argtypes = [vp, ctypes.POINTER(SelectArgs)]
     lib.wamffn_pack_weight.argtypes = [vp, vp, vp, i, i]

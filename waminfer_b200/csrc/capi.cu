@@ -1946,7 +1946,15 @@ struct KvAttnPlan {
   int64_t row_tiles;
 };
 
-KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, int most_parts) {
+// What the plan asks of a device: its SMs, and the clusters of 1 .. 8 CTAs that it holds at once (null: the current
+// device's).
+struct KvAttnDevice {
+  int sm;
+  const int* clusters;
+};
+
+KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, const KvAttnDevice& device, int most_parts) {
+  const int sm = device.sm;
   const int64_t rows = int64_t(p.nq) * p.group;
   KvAttnPlan plan{rows > kFewRows, key_split ? key_split : 1, 1, kManyRows, 1};
   if (plan.many) {
@@ -1965,7 +1973,7 @@ KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, in
       const bool dual = rows <= kManyRows / 2 || tile_rows < kManyRows;
       for (int s = 1; s <= 8; ++s) {
         if (key_split ? s != key_split : 2 * s > std::max<int64_t>(steps, 2)) continue;
-        const int64_t at_once = s == 1 ? sm : many_clusters(s);
+        const int64_t at_once = s == 1 ? sm : device.clusters ? device.clusters[s] : many_clusters(s);
         if (at_once < 1) continue;
         for (int n = 1; n <= most_parts && (n == 1 || 4 * s * n <= steps); ++n) {
           auto cta = [&](int64_t all) {  // time of a CTA
@@ -1992,6 +2000,11 @@ KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, int sm, in
   const int64_t spare = 3 * int64_t(sm) / (ctas * plan.split), busy = units / (4 * kFewWarps * plan.split);
   plan.parts = int(std::max<int64_t>(1, std::min<int64_t>(most_parts, std::min(spare, busy))));
   return plan;
+}
+
+// Parts whose shares the call's workspace holds; one needs none.
+int parts_that_fit(const wamffn_cache_attention_args& a, const KvAttnParams& p) {
+  return a.workspace ? int(std::max<size_t>(1, std::min<size_t>(a.workspace_bytes / part_bytes(p), 32))) : 1;
 }
 
 }  // namespace
@@ -2108,8 +2121,27 @@ int wamffn_cache_attention_workspace(const wamffn_cache_attention_args* a, size_
   KvAttnParams p{};
   int sm = 0, rc = check_cache_attention(a, &p);
   if (rc || (rc = prepare_current_device(&sm))) return rc;
-  KvAttnPlan plan = plan_cache_attention(p, a->key_split, sm, 32);
+  KvAttnPlan plan = plan_cache_attention(p, a->key_split, KvAttnDevice{sm, nullptr}, 32);
   if (plan.parts > 1) *bytes = part_bytes(p) * plan.parts;
+  return WAMFFN_OK;
+}
+
+int wamffn_cache_attention_plan(const wamffn_cache_attention_args* a, wamffn_cache_plan* out) {
+  if (!out) return fail(WAMFFN_ERR_INVALID, "plan is null");
+  KvAttnParams p{};
+  KvAttnDevice device{out->sm_count, out->clusters};
+  int rc = check_cache_attention(a, &p);
+  if (rc) return rc;
+  if (device.sm <= 0) {
+    if ((rc = prepare_current_device(&device.sm))) return rc;
+    device.clusters = nullptr;
+  }
+  const KvAttnPlan plan = plan_cache_attention(p, a->key_split, device, parts_that_fit(*a, p));
+  out->tensor_cores = plan.many;
+  out->key_split = plan.split;
+  out->parts = plan.parts;
+  out->tile_rows = plan.many ? plan.tile_rows : kFewRows;
+  out->row_tiles = plan.row_tiles;
   return WAMFFN_OK;
 }
 
@@ -2121,9 +2153,7 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   if (a->workspace && !aligned16(a->workspace))
     return fail(WAMFFN_ERR_INVALID, "workspace must be a 16-byte aligned pointer");
   if ((rc = prepare_current_device(&sm))) return rc;
-  const size_t part = part_bytes(p);
-  const int most = a->workspace ? int(std::min<size_t>(a->workspace_bytes / part, 32)) : 1;
-  const KvAttnPlan plan = plan_cache_attention(p, a->key_split, sm, most);
+  const KvAttnPlan plan = plan_cache_attention(p, a->key_split, KvAttnDevice{sm, nullptr}, parts_that_fit(*a, p));
   p.split = plan.split;
   p.parts = plan.parts;
   p.tile_rows = plan.tile_rows;
