@@ -58,3 +58,15 @@ def test_the_plan_rejects_what_the_call_rejects():
     assert b"multiple" in lib.wamffn_last_error()
     assert lib.wamffn_cache_attention_plan(None, ctypes.byref(plan)) == 1
     assert lib.wamffn_cache_attention_plan(ctypes.byref(args), None) == 1
+
+
+def test_a_split_that_the_device_cannot_run_is_refused():
+    """No cluster of eight fits: a forced split of eight has no plan, the automatic choice takes another."""
+    none = CLUSTERS[:8] + (0,)
+    args = attention_args(300, 4, 1, 64, key_split=8)
+    plan = _lib.CachePlan(sm_count=148, clusters=(ctypes.c_int * 9)(*none))
+    assert _lib.lib().wamffn_cache_attention_plan(ctypes.byref(args), ctypes.byref(plan)) == 3  # unsupported
+    assert b"key_split=8" in _lib.lib().wamffn_last_error()
+    args = attention_args(300, 4, 1, 64)
+    alone = plan_of(args, (0, 148) + (0,) * 7)
+    assert alone.key_split == 1 and covers(alone, 1200)

@@ -1953,7 +1953,8 @@ struct KvAttnDevice {
   const int* clusters;
 };
 
-KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, const KvAttnDevice& device, int most_parts) {
+int plan_cache_attention(const KvAttnParams& p, int key_split, const KvAttnDevice& device, int most_parts,
+                         KvAttnPlan* out) {
   const int sm = device.sm;
   const int64_t rows = int64_t(p.nq) * p.group;
   KvAttnPlan plan{rows > kFewRows, key_split ? key_split : 1, 1, kManyRows, 1};
@@ -1988,7 +1989,10 @@ KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, const KvAt
         }
       }
     }
-    return plan;
+    if (best == 0)  // the device holds no such cluster, or would not say
+      return fail(WAMFFN_ERR_UNSUPPORTED, "key_split=%d: the device runs no cluster of so many CTAs", key_split);
+    *out = plan;
+    return WAMFFN_OK;
   }
   // Enough CTAs for three an SM, as long as a warp has a unit; and beyond that as
   // long as it has sixteen, so that ragged sequences even out over several waves.
@@ -1999,7 +2003,8 @@ KvAttnPlan plan_cache_attention(const KvAttnParams& p, int key_split, const KvAt
   // Parts as long as SMs are left without a CTA and a warp has four units (about what the second kernel costs).
   const int64_t spare = 3 * int64_t(sm) / (ctas * plan.split), busy = units / (4 * kFewWarps * plan.split);
   plan.parts = int(std::max<int64_t>(1, std::min<int64_t>(most_parts, std::min(spare, busy))));
-  return plan;
+  *out = plan;
+  return WAMFFN_OK;
 }
 
 // Parts whose shares the call's workspace holds; one needs none.
@@ -2121,7 +2126,8 @@ int wamffn_cache_attention_workspace(const wamffn_cache_attention_args* a, size_
   KvAttnParams p{};
   int sm = 0, rc = check_cache_attention(a, &p);
   if (rc || (rc = prepare_current_device(&sm))) return rc;
-  KvAttnPlan plan = plan_cache_attention(p, a->key_split, KvAttnDevice{sm, nullptr}, 32);
+  KvAttnPlan plan;
+  if ((rc = plan_cache_attention(p, a->key_split, KvAttnDevice{sm, nullptr}, 32, &plan))) return rc;
   if (plan.parts > 1) *bytes = part_bytes(p) * plan.parts;
   return WAMFFN_OK;
 }
@@ -2136,7 +2142,8 @@ int wamffn_cache_attention_plan(const wamffn_cache_attention_args* a, wamffn_cac
     if ((rc = prepare_current_device(&device.sm))) return rc;
     device.clusters = nullptr;
   }
-  const KvAttnPlan plan = plan_cache_attention(p, a->key_split, device, parts_that_fit(*a, p));
+  KvAttnPlan plan;
+  if ((rc = plan_cache_attention(p, a->key_split, device, parts_that_fit(*a, p), &plan))) return rc;
   out->tensor_cores = plan.many;
   out->key_split = plan.split;
   out->parts = plan.parts;
@@ -2153,7 +2160,8 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
   if (a->workspace && !aligned16(a->workspace))
     return fail(WAMFFN_ERR_INVALID, "workspace must be a 16-byte aligned pointer");
   if ((rc = prepare_current_device(&sm))) return rc;
-  const KvAttnPlan plan = plan_cache_attention(p, a->key_split, KvAttnDevice{sm, nullptr}, parts_that_fit(*a, p));
+  KvAttnPlan plan;
+  if ((rc = plan_cache_attention(p, a->key_split, KvAttnDevice{sm, nullptr}, parts_that_fit(*a, p), &plan))) return rc;
   p.split = plan.split;
   p.parts = plan.parts;
   p.tile_rows = plan.tile_rows;
