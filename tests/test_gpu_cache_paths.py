@@ -48,3 +48,72 @@ def test_a_workspace_for_less_than_a_part(cuda_device, nq, lengths):
         assert plan_of(args).parts == 1
         run(args)
         close(out, ref, lengths[0])
+
+
+# Two tiles of 128 different rows a CTA (tile_rows 256): several steps, the ring of four stages around more than once,
+# O rescaled; the last tile of at most 128 rows, which runs as one, beside full ones; clusters; parts; ragged batches.
+TWO_TILES = [  # nq, heads, kv_heads, lengths, causal, key_split, parts
+    (670, 32, 8, [513], False, 1, 1),            # 2680 packed rows: a last tile of 120
+    (670, 8, 2, [513, 130], False, 2, 1),        # the same in clusters, ragged
+    (1000, 32, 8, [2000], True, 1, 1),           # 16 tiles, the first rows of a tile see less
+    (400, 24, 24, [700, 1], True, 1, 1),
+    (150, 24, 24, [900, 70], True, 2, 1),
+    (300, 37, 37, [2048], False, 2, 1),          # 300 rows: a last tile of 44
+    (392, 16, 4, [2048], False, 4, 1),
+    (300, 8, 2, [900], True, 8, 1),
+    (128, 32, 8, [4096], False, 8, 1),
+    (392, 24, 24, [9000], False, 1, 2),          # parts through the workspace
+]
+
+
+@pytest.mark.parametrize("nq,heads,kv_heads,lengths,causal,key_split,parts", TWO_TILES)
+def test_two_tiles_of_rows(cuda_device, nq, heads, kv_heads, lengths, causal, key_split, parts):
+    cache, g = make(cuda_device, nq + heads, len(lengths), kv_heads, lengths, spread=3, extra=1)
+    q = rows(g, len(lengths), nq, heads * DIM)
+    out = cache.attend(q, heads, causal=causal, key_split=key_split)
+    workspace = torch.empty(max(cache._needs.values()) or 16, dtype=torch.uint8, device=cuda_device)
+    plan = plan_of(call(cache, q, heads, out, causal, key_split, workspace))
+    assert plan.tile_rows == 256 and plan.key_split == key_split and min(plan.parts, 2) == parts
+    close(out, attention(Model(cache), q, heads, causal), max(lengths))
+    for _ in range(5):
+        assert torch.equal(out, cache.attend(q, heads, causal=causal, key_split=key_split))
+    assert cache.status() == 0
+
+
+def test_one_tile_of_rows_in_parts(cuda_device):
+    """Tiles of 128 rows, each over parts of the keys."""
+    cache, g = make(cuda_device, 396, 1, 4, [9000], spread=3, extra=1)
+    q = rows(g, 1, 392, 4 * DIM)
+    out = cache.attend(q, 4, key_split=1)
+    workspace = torch.empty(max(cache._needs.values()), dtype=torch.uint8, device=cuda_device)
+    plan = plan_of(call(cache, q, 4, out, key_split=1, workspace=workspace))
+    assert plan.tile_rows == 128 and plan.parts > 1
+    close(out, attention(Model(cache), q, 4, False), 9000)
+
+
+def test_two_tiles_of_rows_in_many_parts(cuda_device):
+    """128 rows of 40 heads over 32768 rows of 8: checked at some of the queries."""
+    cache, g = make(cuda_device, 40, 1, 8, [32768], spread=2)
+    q = rows(g, 1, 128, 40 * DIM)
+    out = cache.attend(q, 40)
+    workspace = torch.empty(max(cache._needs.values()), dtype=torch.uint8, device=cuda_device)
+    plan = plan_of(call(cache, q, 40, out, workspace=workspace))
+    assert plan.tile_rows == 256 and plan.parts > 1
+    some = [0, 25, 26, 51, 76, 102, 127]  # around the tiles' borders, and the last tile of 128 rows
+    close(out[:, some], attention(Model(cache), q[:, some], 40, False), 32768)
+
+
+def test_clusters_of_every_size(cuda_device):
+    """Clusters that key_split does not force (3, 5, 6, 7) come from the plan; which shapes take them depends a
+    little on the device, so a spread of shapes stands for them."""
+    found = set()
+    for nq, heads, kv_heads, keys in ((300, 32, 8, 1024), (150, 32, 8, 512), (150, 24, 24, 2048), (65, 32, 8, 2048),
+                                      (300, 16, 4, 3000), (200, 10, 5, 1024), (300, 8, 1, 2048), (200, 8, 1, 2048),
+                                      (250, 8, 1, 2048)):
+        cache, g = make(cuda_device, nq + heads, 1, kv_heads, [keys], spread=2)
+        q = rows(g, 1, nq, heads * DIM)
+        out = cache.attend(q, heads)
+        plan = plan_of(call(cache, q, heads, out))
+        found.add((plan.tile_rows, plan.key_split))
+        close(out, attention(Model(cache), q, heads, False), keys)
+    assert len({split for _, split in found} & {3, 5, 6, 7}) >= 2 and {rows_ for rows_, _ in found} == {128, 256}, found
