@@ -117,3 +117,23 @@ def test_clusters_of_every_size(cuda_device):
         found.add((plan.tile_rows, plan.key_split))
         close(out, attention(Model(cache), q, heads, False), keys)
     assert len({split for _, split in found} & {3, 5, 6, 7}) >= 2 and {rows_ for rows_, _ in found} == {128, 256}, found
+
+
+def test_the_tensors_of_a_cache_are_not_replaced(cuda_device):
+    """Calls go by the tensors that the cache was made of: another one in an attribute's place is refused, not
+    ignored.  In place they change as ever."""
+    cache, g = make(cuda_device, 1, 2, 1, [70, 3], spread=1)
+    q = rows(g, 2, 1, DIM)
+    for name in ("keys", "values", "key_scales", "value_scales", "block_table", "lengths"):
+        old = getattr(cache, name)
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, old.clone())
+        with pytest.raises(AttributeError, match=name):
+            delattr(cache, name)
+        assert getattr(cache, name) is old
+    for name in ("batch", "width", "kv_heads", "device"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, 5)
+    cache.lengths -= 1
+    assert cache.lengths.tolist() == [69, 2]
+    close(cache.attend(q, 1), attention(Model(cache), q, 1, False), 70)

@@ -119,7 +119,9 @@ class KVCache8:
     ``key_scales``, ``value_scales`` float32 [blocks, kv_heads], powers of two from
     2^-60 (a row is value * scale; of another number only the exponent counts);
     ``block_table``; ``lengths`` int32 [batch], rows held (lowering an entry drops
-    rows).  Appends to one cache must not overlap in time with other calls on it.
+    rows).  They are written into, not replaced: the calls go by where they lie, so
+    the attributes cannot be bound anew.  Appends to one cache must not overlap in time
+    with other calls on it.
     """
 
     def __init__(self, batch: int, capacity: int, kv_heads: int, device, blocks: int | None = None):
@@ -175,6 +177,15 @@ class KVCache8:
         self._needs: dict[tuple, int] = {}  # workspace of the attention, by its sizes
         self._work = torch.zeros(batch + 1, dtype=torch.int32, device=device) if work is None else work
         self._view = _layout(keys, values, key_scales, value_scales, block_table, lengths, self._work)
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__ and value is not self.__dict__[name]:  # x += 1 binds the same tensor again
+            raise AttributeError(f"{name} of a cache cannot be replaced: write into it, or make another cache "
+                                 "(KVCache8.of)")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{name} of a cache cannot be deleted")
 
     def _tensors(self):
         return (self.keys, self.values, self.key_scales, self.value_scales, self.block_table, self.lengths, self._work)
