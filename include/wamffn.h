@@ -581,7 +581,9 @@ int wamffn_qk_norm_rope(void* stream, const wamffn_qk_rope_args* args);
  * prefix is bf16, WAMInfer/_triton_attention.py:337-484).  Blocks of
  * WAMFFN_CACHE_BLOCK tokens, head dim 128:
  *   keys, values   [blocks, kv_heads, 64, 128] e4m3, 16-byte aligned
- *   *_scales       [blocks, kv_heads] fp32, powers of two; a row is value * scale
+ *   *_scales       [blocks, kv_heads] fp32, powers of two from 2^-60 to 2^126 (of
+ *                  another number the exponent counts, cut to that range); a
+ *                  row is value * scale
  *   block_table    [batch, width] int32 (table_stride elements between
  *                  sequences): the block of rows [64 i, 64 i + 64)
  *   lengths        [batch] int32, rows held

@@ -137,3 +137,29 @@ def test_the_tensors_of_a_cache_are_not_replaced(cuda_device):
     cache.lengths -= 1
     assert cache.lengths.tolist() == [69, 2]
     close(cache.attend(q, 1), attention(Model(cache), q, 1, False), 70)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 120, 2.0 ** 126, 2.0 ** 127, float("inf"), float("nan")])
+def test_the_largest_scales(cuda_device, scale):
+    """A value block of the largest scale that counts, 2^126, and of scales past it: read, attended, appended to."""
+    cache, g = make(cuda_device, 8, 1, 2, [80], capacity=192, spread=1)
+    small = torch.randn(cache.values.shape, device=cuda_device, generator=g).clamp(-1, 1)  # results stay finite
+    cache.values.copy_(torch.where(cache.values.float().isnan(), float("nan"), small).to(torch.float8_e4m3fn))
+    cache.value_scales.fill_(scale)
+    model = Model(cache)
+    model.exps[1].fill_(120 if scale == 2.0 ** 120 else 126)
+    for nq, causal in ((1, True), (9, False), (70, True), (300, False)):
+        q = rows(g, 1, nq, 2 * DIM)
+        close(cache.attend(q, 2, causal=causal), attention(model, q, 2, causal), 80)
+    v = cache.read(80)[1][0]
+    for h in range(2):
+        assert torch.equal(v[:, h * DIM:(h + 1) * DIM].cpu().double(), model.rows(1, 0, h))
+    new = rows(g, 1, 3, 2 * DIM)
+    new[0, 0, :6] = torch.tensor([2.0 ** 126, -3e38, float("inf"), -float("inf"), float("nan"), 2.0 ** 117])
+    cache.append(new, new)
+    model.append(new, new)
+    assert cache.status() == 0 and cache.lengths.tolist() == [83]
+    held = cache.values[cache.block_table[0, 1].long()].cpu().double()
+    assert torch.equal(held[:, :19].nan_to_num(1e9), model.codes[1][model.table[0][1], :, :19].nan_to_num(1e9))
+    assert torch.equal(torch.log2(cache.value_scales[cache.block_table[0, 1].long()].cpu().double()),
+                       model.exps[1][model.table[0][1]])

@@ -117,7 +117,8 @@ class KVCache8:
 
     Tensors: ``keys``, ``values`` [blocks, kv_heads, 64, 128] float8_e4m3fn;
     ``key_scales``, ``value_scales`` float32 [blocks, kv_heads], powers of two from
-    2^-60 (a row is value * scale; of another number only the exponent counts);
+    2^-60 to 2^126 (a row is value * scale; of another number only the exponent
+    counts, cut to that range);
     ``block_table``; ``lengths`` int32 [batch], rows held (lowering an entry drops
     rows).  They are written into, not replaced: the calls go by where they lie, so
     the attributes cannot be bound anew.  Appends to one cache must not overlap in time

@@ -27,7 +27,9 @@ namespace wamffn {
 constexpr int kCacheBlock = 64;   // tokens of a block
 constexpr int kCacheDim = 128;    // head dim
 constexpr int kCacheTile = kCacheBlock * kCacheDim;  // bytes of a (block, head) tile
-constexpr int kCacheLeastExp = -60;
+// A scale's exponent: from -60 (the store's floor; 2^eq 2^ek of a query and a block stays normal) to 126 (its
+// reciprocal is a normal number; the store never makes more than 120).
+constexpr int kCacheLeastExp = -60, kCacheMostExp = 126;
 
 struct CacheView {
   uint8_t *keys, *values;
@@ -69,9 +71,9 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 }
 // 2^e, -126 <= e <= 127.
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
-// The exponent of a stored scale (a power of two).
+// The exponent of a stored scale (a power of two; infinities and NaN count as the largest).
 __device__ __forceinline__ int scale_exp(float s) {
-  return max(kCacheLeastExp, min(127, ((__float_as_int(s) >> 23) & 255) - 127));
+  return max(kCacheLeastExp, min(kCacheMostExp, ((__float_as_int(s) >> 23) & 255) - 127));
 }
 // e(block) from the largest finite |x| as bf16 bits: the least e with |x| <= 448 * 2^e = 1.75 * 2^(e + 8).
 __device__ __forceinline__ int cache_exp(uint32_t bits) {
