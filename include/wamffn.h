@@ -652,7 +652,9 @@ int wamffn_cache_read(void* stream, const wamffn_cache_read_args* args);
  * that sees nothing is zeros.  q: [batch, nq, heads * 128] bf16 (strides
  * multiples of 8), heads a multiple of the cache's kv_heads: query heads
  * [g * heads / kv_heads, ...) share key head g.  out contiguous.  fp32 scores,
- * maximum, sums; the probabilities of the value product in f16.  A block id
+ * maximum, sums, every key counted in the normaliser whatever its values' scale;
+ * the probabilities of the value product in f16 with that scale: full precision
+ * down to 2^-19 of the row's largest such product, steps of 2^-29 of it below.  A block id
  * outside the pool is left out and sets WAMFFN_DEV_BAD_INDEX.  key_split: CTAs
  * of a cluster that share a row tile's keys, 0 picks it (1, 2, 4 or 8 forces it).
  * Few row tiles over long sequences are also cut into parts whose shares a second

@@ -163,3 +163,102 @@ def test_the_largest_scales(cuda_device, scale):
     assert torch.equal(held[:, :19].nan_to_num(1e9), model.codes[1][model.table[0][1], :, :19].nan_to_num(1e9))
     assert torch.equal(torch.log2(cache.value_scales[cache.block_table[0, 1].long()].cpu().double()),
                        model.exps[1][model.table[0][1]])
+
+
+def close_held(cache, got, q, heads, keys):
+    """The module's tolerance and what it leaves out: the probabilities times the scale of their values, P, are f16
+    numbers with a row's largest at 2^5 or more.  Below 2^-14 they are off by up to 2^-25, so by 2^-30 of the largest,
+    and the sum over the values (codes, without their scale) by that times sum |code|."""
+    model = Model(cache)
+    out, absolute, bound = attention(model, q, heads, False)
+    batch, nq, _ = q.shape
+    group = heads // cache.kv_heads
+    extra = torch.zeros(batch, nq, heads, DIM, dtype=torch.float64)
+    for b in range(batch):
+        n = model.lengths[b]
+        ids = model.table[b][:-(-n // 64)]
+        for h in range(heads):
+            s = q[b].cpu().double().view(nq, heads, DIM)[:, h] @ model.rows(0, b, h // group).T / DIM ** 0.5
+            p = torch.softmax(s, -1)
+            scale = torch.exp2(model.exps[1][ids, h // group]).repeat_interleave(64)[:n]
+            codes = model.codes[1][ids, h // group].reshape(-1, DIM)[:n].abs().nan_to_num().sum(0)
+            extra[b, :, h] = 2.0 ** -30 * (p * scale).amax(-1, keepdim=True) * codes
+    got = got.cpu().double()
+    assert got.isfinite().all()
+    tol = 2.0 ** -8 * out.abs() + (2.0 ** -11 + 2 * 2.0 ** -16 * bound + keys * 2.0 ** -23 + 2.0 ** -20) * absolute
+    off = (got - out).abs() - tol - extra.flatten(2)
+    assert off.max().item() <= 0, (off.max().item(), tol.flatten()[off.argmax()].item())
+
+
+def far_apart(cache, g, huge, zero, exponent):
+    """Ordinary keys and values; block `huge` of the first sequence holds values of 2^exponent, block `zero` none."""
+    ids = cache.block_table[0].long()
+    cache.value_scales.fill_(2.0 ** -6)
+    cache.value_scales[ids[huge]] = 2.0 ** (exponent - 6)
+    cache.value_scales[ids[zero]] = 2.0 ** -60
+    cache.values.view(torch.uint8)[ids[zero]] = 0
+    return ids
+
+
+# Every place where shares of a row meet: steps of a warp or a tile, warps, the two tiles of the same rows, a cluster,
+# parts through the workspace.
+MEETINGS = [  # nq, heads, kv_heads, length, key_split
+    (1, 2, 1, 128, 1),
+    (1, 8, 2, 1100, 0),
+    (12, 1, 1, 128, 0),
+    (5, 3, 1, 1500, 4),
+    (1, 1, 1, 9000, 0),
+    (40, 2, 2, 128, 1),
+    (40, 2, 2, 700, 8),
+    (130, 1, 1, 9000, 0),
+    (300, 24, 24, 448, 1),
+    (300, 16, 4, 1024, 2),
+]
+
+
+@pytest.mark.parametrize("exponent", [75, 100, 125])
+@pytest.mark.parametrize("nq,heads,kv_heads,length,key_split", MEETINGS)
+def test_a_block_of_zeros_beside_one_of_huge_values(cuda_device, nq, heads, kv_heads, length, key_split, exponent):
+    """All keys keep their share of the normaliser, however far apart the scales of their values lie."""
+    cache, g = make(cuda_device, nq + exponent, 1, kv_heads, [length])
+    q = rows(g, 1, nq, heads * DIM)
+    q[:, ::2] = 0  # equal scores
+    blocks = cache.width
+    for huge, zero in ((0, 1), (1, 0), (blocks - 1, blocks // 2), (blocks // 2, blocks - 1)):
+        if huge != zero:
+            far_apart(cache, g, huge, zero, exponent)
+            close_held(cache, cache.attend(q, heads, key_split=key_split), q, heads, length)
+            cache.values.copy_(torch.where(cache.values.float() == 0, 40.0, cache.values.float()).to(cache.values.dtype))
+
+
+@pytest.mark.parametrize("exponent", [40, 80, 110])
+@pytest.mark.parametrize("nq,heads,kv_heads,length,key_split", MEETINGS)
+def test_huge_values_at_low_scores(cuda_device, nq, heads, kv_heads, length, key_split, exponent):
+    """Keys whose weight is about 2^-exponent of the others' and whose values are 2^exponent of theirs count as much;
+    the queries before and behind those that see it so give them more and less."""
+    cache, g = make(cuda_device, nq + exponent, 1, kv_heads, [length])
+    blocks = cache.width
+    q = torch.zeros(1, nq, heads * DIM, device=cuda_device)
+    q.view(1, nq, heads, DIM)[..., 0] = torch.linspace(0.8, 1.2, nq, device=cuda_device)[None, :, None]
+    q += torch.randn(q.shape, device=cuda_device, generator=g) * 2.0 ** -8
+    q = q.bfloat16()
+    for huge, zero in ((0, 1), (1, 0), (blocks - 1, blocks // 2)):
+        if huge == zero:
+            continue
+        ids = far_apart(cache, g, huge, zero, exponent)
+        cache.key_scales.fill_(2.0 ** -6)
+        cache.key_scales[ids[huge]] = 2.0  # dim 0 of these keys: -ln(2) * exponent * sqrt(128)
+        keys = cache.keys.float().clamp(-100, 100)
+        keys[ids[huge], :, :, 0] = -exponent * 0.6931 * 128 ** 0.5 / 2
+        keys[ids[huge], :, :, 1:] = 0
+        cache.keys.copy_(keys.to(cache.keys.dtype))
+        cache.values.copy_(torch.where(cache.values.float().abs() > 64, 3.0, cache.values.float()).to(cache.values.dtype))
+        close_held(cache, cache.attend(q, heads, key_split=key_split), q, heads, length)
+
+
+@pytest.mark.parametrize("nq,heads,kv_heads,length,key_split", MEETINGS)
+def test_sharp_scores(cuda_device, nq, heads, kv_heads, length, key_split):
+    """Blocks hundreds of binades below a row's maximum, before and behind it."""
+    cache, g = make(cuda_device, nq, 1, kv_heads, [length], spread=3)
+    q = rows(g, 1, nq, heads * DIM, size=24.0)
+    close_held(cache, cache.attend(q, heads, key_split=key_split), q, heads, length)

@@ -16,6 +16,11 @@
 //   (full precision down to 2^-19 of the largest, steps of 2^-29 of it below);
 //   P V adds up to the numerator, sum_j P_j 2^-ev (fp32, before P is rounded) to the
 //   denominator, and 2^(5 - m) cancels.
+//   The denominator counts every key, whatever its values' scale: of 64 zeros (ev -60) beside values of 1e23 too,
+//   whose x differ by more than fp32's exponents reach.  So where a row's x lie 2^100 and more below m throughout a
+//   unit or step, P is taken against their own maximum, only for the sum (f16 has zeros for them anyway), which then
+//   gets the difference; and a change of m takes the denominator along as two factors (folded).  The sum itself stays
+//   between 2^(5 - ev) of the largest x's ev and 2^(13 - ev) of the smallest, so within 2^-121 .. 2^73 a key.
 //
 // Masked keys have x = -inf.  Rows past a sequence's length are whatever the
 // block held before; they, and NaN in a value that only some rows of a tile see,
@@ -57,6 +62,9 @@ __device__ __forceinline__ void kv_emit(const KvAttnParams& p, int part, int b, 
   }
 }
 
+// x times h^2, where h^2 may be too small for a float and x too large.
+__device__ __forceinline__ float folded(float x, float h) { return x * h * h; }
+
 // The parts' shares of a row in their order; a warp a row.
 constexpr int kMergeThreads = 256;
 __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvAttnParams p, long long rows) {
@@ -71,10 +79,11 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvAttnPar
     const float2 ml = p.part_ml[k * rows + row];
     const float4 u = *reinterpret_cast<const float4*>(p.part_o + (k * rows + row) * kCacheDim + d);
     const float next = fmaxf(top, ml.x), safe = next == -INFINITY ? 0.f : next;
-    const float fo = ex2_approx(top - safe), fn = ex2_approx(ml.x - safe);
+    const float ho = ex2_approx(0.5f * (top - safe)), hn = ex2_approx(0.5f * (ml.x - safe));
+    const float fo = ho * ho, fn = hn * hn;
     v.x = v.x * fo + u.x * fn, v.y = v.y * fo + u.y * fn;
     v.z = v.z * fo + u.z * fn, v.w = v.w * fo + u.w * fn;
-    sum = sum * fo + ml.y * fn;
+    sum = folded(sum, ho) + folded(ml.y, hn);
     top = next;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -83,6 +92,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvAttnPar
 }
 
 constexpr float kPBias = 5.f, kLag = 8.f;  // P <= 2^(5 + 8)
+constexpr float kDeep = 100.f;             // x below m by this: P - 31 binades of it are still normal numbers
 
 __device__ __forceinline__ uint32_t f16x2_pack(float lo, float hi) {
   uint32_t d;
@@ -408,21 +418,19 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
           x[j][e] = v;
           top[slot(e)] = fmaxf(top[slot(e)], v);
         }
-      float base[2], corr[2];
-      bool grown = false;
+      // A maximum that grows by at most 2^kLag is left as it is: P stays below f16's range.
+      bool apart[2];
+      float base[2], sum[2] = {0.f, 0.f}, back[2] = {exp2_int(-ev), exp2_int(-ev)};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int w = kNarrow ? 4 : 1; w < (kNarrow ? 32 : 4); w <<= 1)
           top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], w));
-        // A maximum that grows by at most 2^kLag is left as it is: P stays below f16's range.
-        const bool g = top[half] > m[half] + kLag || (m[half] == -INFINITY && top[half] > m[half]);
-        corr[half] = g ? ex2_approx(m[half] - top[half]) : 1.f;
-        grown |= g;
-        if (g) m[half] = top[half];
-        base[half] = kPBias - (m[half] == -INFINITY ? 0.f : m[half]);
+        apart[half] = top[half] > -INFINITY &&
+                      (top[half] > m[half] + kLag || top[half] < m[half] - kDeep || m[half] == -INFINITY);
+        const float ref = apart[half] ? top[half] : m[half];
+        base[half] = kPBias - (ref == -INFINITY ? 0.f : ref);
       }
-      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
@@ -430,15 +438,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
           x[j][e] = ex2_approx(x[j][e] + base[slot(e)]);
           sum[slot(e)] += x[j][e];
         }
-      const float back = exp2_int(-ev);
-      l[0] = fmaf(sum[0], back, l[0] * corr[0]);
-      l[1] = fmaf(sum[1], back, l[1] * corr[1]);
-      if (__any_sync(0xffffffffu, grown)) {
+      if (__any_sync(0xffffffffu, apart[0] || apart[1])) {
+        float corr[2], keep[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          corr[half] = keep[half] = 1.f;
+          if (apart[half]) {
+            const bool grown = top[half] > m[half];
+            const float fold = ex2_approx(0.5f * (grown ? m[half] - top[half] : top[half] - m[half] - evf));
+            if (grown) {
+              corr[half] = fold * fold;
+              l[half] = folded(l[half], fold);
+              m[half] = top[half];
+            } else {  // deep: the sum alone gets these
+              keep[half] = 0.f;
+              back[half] = fold;
+              sum[half] *= fold;
+            }
+          }
+        }
 #pragma unroll
         for (int n = 0; n < (kNarrow ? 8 : 16); ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[n][e] *= corr[slot(e)];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][e] *= keep[slot(e)];
       }
+      l[0] = fmaf(sum[0], back[0], l[0]);
+      l[1] = fmaf(sum[1], back[1], l[1]);
       // O += P V, 16 keys a step.
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -523,11 +552,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < kFewWarps; ++k) {
-      const float f = ex2_approx(part_ml[k][r].x - safe);
+      const float fold = ex2_approx(0.5f * (part_ml[k][r].x - safe)), f = fold * fold;
       const float4 u = *reinterpret_cast<const float4*>(
           reinterpret_cast<const float*>(ring + k * kFewRing) + r * kFewPitch + d);
       v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
-      sum += part_ml[k][r].y * f;
+      sum += folded(part_ml[k][r].y, fold);
     }
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(ring) + r * kFewPitch + d) = v;
     if (d == 0) cta_ml[r] = make_float2(top, sum);
@@ -560,9 +589,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
     const float safe = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float f = ex2_approx(ml[k].x - safe);
+      const float fold = ex2_approx(0.5f * (ml[k].x - safe)), f = fold * fold;
       v.x += u[k].x * f, v.y += u[k].y * f, v.z += u[k].z * f, v.w += u[k].w * f;
-      sum += ml[k].y * f;
+      sum += folded(ml[k].y, fold);
     }
     const int token = r / p.group, head = kh * p.group + r - token * p.group;
     if (!abort_flag) kv_emit(p, part, b, token, head, d, v, top, sum);

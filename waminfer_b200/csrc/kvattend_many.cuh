@@ -447,11 +447,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         const bool grown = top > m + kLag || (m == -INFINITY && top > m);
         float corr = 1.f;
         if (grown) {
-          corr = ex2_approx(m - top);
+          const float fold = ex2_approx(0.5f * (m - top));
+          corr = fold * fold;
           m = top;
-          l *= corr;
+          l = folded(l, fold);
         }
-        const float base = sc.ev - (m == -INFINITY ? 0.f : m) + kPBias;
+        const bool deep = top < m - kDeep && top > -INFINITY;
+        const bool rare = __any_sync(0xffffffffu, grown || deep);
+        const float ref = deep ? top : m;
+        const float base = sc.ev - (ref == -INFINITY ? 0.f : ref) + kPBias;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t out[32];
 #pragma unroll
@@ -463,9 +467,21 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           sum[i & 1] = add2(sum[i & 1], e);
           out[i] = f16x2_pack(e.x, e.y);
         }
+        float back = sc.back;
+        if (rare) {
+          if (deep) {  // the sum alone gets these (kvattend.cuh)
+            const float fold = ex2_approx(0.5f * (top - m - sc.ev));
+            back = fold;
+            sum[0] = make_float2((sum[0].x + sum[1].x) * fold, (sum[0].y + sum[1].y) * fold);
+            sum[1] = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) out[i] = 0u;
+          }
+          __syncwarp();
+        }
         tmem_st32(ts, out);
-        l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), sc.back, l);
-        if (__any_sync(0xffffffffu, grown) && n > 0) {
+        l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), back, l);
+        if (rare && n > 0 && __any_sync(0xffffffffu, grown)) {
           if (lane == 0)
             ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(n - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
           ok = warp_verdict(ok);
@@ -542,10 +558,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
       named_sync(1, kManySoftmaxWarps * 32);
       const float2 e0 = held_ml[rr], e1 = held_ml[rr + 128];
       const float top = fmaxf(e0.x, e1.x), safe = top == -INFINITY ? 0.f : top;
-      const float f0 = ex2_approx(e0.x - safe), f1 = ex2_approx(e1.x - safe);
-      f = x ? f1 : f0;
+      const float h0 = ex2_approx(0.5f * (e0.x - safe)), h1 = ex2_approx(0.5f * (e1.x - safe));
+      f = x ? h1 * h1 : h0 * h0;
       m = top;
-      l = e0.y * f0 + e1.y * f1;
+      l = folded(e0.y, h0) + folded(e1.y, h1);
 #pragma unroll 1
       for (int q = x ? 0 : 2, n = 0; n < 2; ++n, ++q) {
         uint32_t v[32];
@@ -625,9 +641,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
             const float safe = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int k = 0; k < kShares; ++k) {
-              const float fk = ex2_approx(ml[n][k].x - safe);
+              const float fold = ex2_approx(0.5f * (ml[n][k].x - safe)), fk = fold * fold;
               v.x += u[n][k].x * fk, v.y += u[n][k].y * fk, v.z += u[n][k].z * fk, v.w += u[n][k].w * fk;
-              sum += ml[n][k].y * fk;
+              sum += folded(ml[n][k].y, fold);
             }
             const int i = i0 + n * kManySoftmaxWarps * 32, prow = row0 + rank + (i >> 5) * split;
             const int ptoken = prow / p.group, phead = kh * p.group + prow - ptoken * p.group;
