@@ -115,7 +115,7 @@ __device__ __forceinline__ void rope_store(__nv_bfloat16* head, const RopeDims& 
   for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
   // Pairs inside the lane: (0,1)(2,3)(4,5)(6,7) interleaved, (0,4)(1,5)(2,6)(3,7) in halves.
   // An unturned lane's dims are no pairs: an infinity or NaN of one must not reach the other (0 x inf).
-  // (Selects: 56.4 us in the header's first case, a branch around the products 57.6.)
+  // (Selects cost 0.3 us of 56 called in the prompt case above, a branch around the products 1.5.)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int a = kInterleaved ? 2 * i : i, b = kInterleaved ? 2 * i + 1 : i + 4;

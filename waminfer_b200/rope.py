@@ -160,8 +160,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     outside the table gives a row of NaN.  head_dim 64, 128 or 256.  ``k`` may
     be None (a cross-attention query).
     """
-    if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (k is not None and (
-            k.requires_grad or (k_weight is not None and k_weight.requires_grad)))):
+    if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (
+            rope is not None and rope.requires_grad) or (k is not None and (
+                k.requires_grad or (k_weight is not None and k_weight.requires_grad)))):
         raise RuntimeError("qk_norm_rope has no backward pass: run it with gradients disabled")
     if k is not None and torch.compiler.is_compiling():
         return _op(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved)
