@@ -262,3 +262,24 @@ def test_sharp_scores(cuda_device, nq, heads, kv_heads, length, key_split):
     cache, g = make(cuda_device, nq, 1, kv_heads, [length], spread=3)
     q = rows(g, 1, nq, heads * DIM, size=24.0)
     close_held(cache, cache.attend(q, heads, key_split=key_split), q, heads, length)
+
+
+def test_recorded_on_tensors_with_data(cuda_device):
+    """A tracer outside the compiler records the calls instead of their results."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from waminfer_b200.cache import KVCache8
+
+    caches = [KVCache8(2, 128, 1, cuda_device) for _ in range(2)]
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    at = torch.zeros(2, dtype=torch.int32, device=cuda_device)
+
+    def step(cache, x):
+        cache.append(x[..., :DIM], x[..., DIM:], at=at)
+        return cache.attend(x, 2, causal=True), *cache.read(5)
+
+    x, y = rows(g, 2, 5, 2 * DIM), rows(g, 2, 5, 2 * DIM)
+    recorded = make_fx(lambda x: step(caches[0], x))(x)
+    for a, b in zip(recorded(y), step(caches[1], y)):
+        assert torch.equal(a, b)
+    assert torch.equal(caches[0].keys.view(torch.uint8), caches[1].keys.view(torch.uint8))

@@ -34,3 +34,30 @@ def test_special_values_stay_in_their_pair(cuda_device, dim, pairs, interleaved,
     assert torch.equal(torch.where(got.isinf(), got, 0.0), torch.where(y.isinf(), y, 0.0))
     off = torch.where(y.isfinite(), (got - y).abs() - (2.0 ** -8 * y.abs() + 2.0 ** -20 * size), 0.0)
     assert off.nan_to_num(1.0).max().item() <= 0
+
+
+def test_queries_alone_traced(cuda_device):
+    """The cross-attention form inside a compiled function, with and without a table, and recorded by a tracer on
+    tensors with data."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from waminfer_b200.rope import qk_norm_rope
+
+    q, k, qw, kw, g = case(cuda_device, 4, 2, 7, 4, 2, 128, False)
+    freqs = table(20, 64, cuda_device)
+    positions = torch.randint(0, 20, (2, 7), device=cuda_device, generator=g)
+
+    def step(q):
+        return (qk_norm_rope(q, None, qw, None, freqs, positions, 4, eps=1e-5)[0],
+                qk_norm_rope(q, None, qw, None, None, None, 4)[0] * 1.0,
+                *qk_norm_rope(q, k, qw, kw, freqs, None, 4, 2, interleaved=False))
+
+    with torch.no_grad():
+        plain = step(q)
+        traced = torch.compile(step, backend="aot_eager", fullgraph=True)(q)
+        recorded = make_fx(step)(q)
+        other = torch.randn(q.shape, device=cuda_device, generator=g).bfloat16()
+        again = recorded(other)
+        expect = step(other)
+    for a, b in zip((*plain, *expect), (*traced, *again)):
+        assert torch.equal(a, b)

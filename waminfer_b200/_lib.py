@@ -392,6 +392,12 @@ def check(status: int) -> None:
         raise WamffnError(status, message)
 
 
+def traced(t: torch.Tensor, compiling=torch.compiler.is_compiling, modes=torch._C._len_torch_dispatch_stack,
+           recorded=torch._C._is_tracing, plain=torch.Tensor) -> bool:
+    """Whether a call on t is being traced, or has no data to run on: it then goes through its op."""
+    return compiling() or type(t) is not plain or modes() > 0 or recorded()
+
+
 def launch(entry, device: int, args) -> None:
     """Calls entry(current stream of `device`, args) with `device` current."""
     if torch._C._cuda_getDevice() == device:

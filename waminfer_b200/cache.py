@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 
 from waminfer_b200 import _lib
 
@@ -177,7 +178,8 @@ class KVCache8:
         self.batch, self.width, self.kv_heads, self.device = batch, width, kv_heads, device
         self._needs: dict[tuple, int] = {}  # workspace of the attention, by its sizes
         self._work = torch.zeros(batch + 1, dtype=torch.int32, device=device) if work is None else work
-        self._view = _layout(keys, values, key_scales, value_scales, block_table, lengths, self._work)
+        self._view = None if isinstance(keys, FakeTensor) else _layout(  # without data there are no addresses
+            keys, values, key_scales, value_scales, block_table, lengths, self._work)
 
     def __setattr__(self, name, value):
         if name in self.__dict__ and value is not self.__dict__[name]:  # x += 1 binds the same tensor again
@@ -214,7 +216,7 @@ class KVCache8:
         rounded to the new one.  A sequence whose rows do not fit (past capacity, ``at``
         beyond its length, a block id outside the pool) keeps what it had, and
         ``status`` reports it."""
-        if torch.compiler.is_compiling():
+        if _lib.traced(k):
             return _append_op(k, v, counts, at, *self._tensors())
         self._append(k, v, counts, at)
 
@@ -234,7 +236,7 @@ class KVCache8:
         """Rows [start, start + count) of every sequence as bf16, k and v
         [batch, count, kv_heads * 128]; ``start`` a number or int32 [batch].
         Rows that a sequence does not hold are zeros."""
-        if torch.compiler.is_compiling():
+        if _lib.traced(self.keys):
             tensor = isinstance(start, torch.Tensor)
             return _read_op(count, start if tensor else None, 0 if tensor else start, *self._tensors())
         return self._read(count, start)
@@ -259,7 +261,7 @@ class KVCache8:
         row that sees nothing is zeros.  NaN comes out where a row sees it: of a
         query or key in the whole of its heads, of a value in its dim.  key_split:
         CTAs of a cluster sharing a query tile's keys (0 = chosen; 1, 2, 4, 8)."""
-        if torch.compiler.is_compiling():
+        if _lib.traced(q):
             return _attend_op(q, heads, causal, key_split, *self._tensors())
         return self._attend(q, heads, causal, key_split)
 

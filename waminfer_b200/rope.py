@@ -144,6 +144,17 @@ def _fake(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, inter
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
+@torch.library.custom_op("wam_ffn::q_norm_rope", mutates_args=())
+def _alone_op(q: torch.Tensor, q_weight: torch.Tensor, rope: torch.Tensor | None, positions: torch.Tensor | None,
+              heads: int, eps: float, interleaved: bool) -> torch.Tensor:
+    return _run(q, None, q_weight, None, rope, positions, heads, 0, eps, interleaved)[0]
+
+
+@_alone_op.register_fake
+def _alone_fake(q, q_weight, rope, positions, heads, eps, interleaved):
+    return q.new_empty(q.shape)
+
+
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor, k_weight: torch.Tensor | None,
                  rope: torch.Tensor | None, positions: torch.Tensor | None, heads: int, kv_heads: int = 0,
                  eps: float = 1e-6, interleaved: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:
@@ -164,6 +175,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
             rope is not None and rope.requires_grad) or (k is not None and (
                 k.requires_grad or (k_weight is not None and k_weight.requires_grad)))):
         raise RuntimeError("qk_norm_rope has no backward pass: run it with gradients disabled")
-    if k is not None and torch.compiler.is_compiling():
+    if _lib.traced(q):
+        if k is None:
+            return _alone_op(q, q_weight, rope, positions, heads, eps, interleaved), None
+        if k_weight is None:
+            raise ValueError("k needs k_weight")
         return _op(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved)
     return _run(q, k, q_weight, k_weight, rope, positions, heads, kv_heads, eps, interleaved)
