@@ -17,3 +17,14 @@ def test_the_verdict_of_a_wait_reaches_the_warp_with_its_memory(name):
     assert text.count("warp_verdict(") >= 4
     helper = (CSRC / "ptx.cuh").read_text().split("int warp_verdict(int found) {")[1].split("\n}")[0]
     assert helper.index("__shfl_sync") < helper.index("__syncwarp();")
+
+
+def test_one_kernel_s_build_does_not_decide_over_the_library():
+    """A kernel that a compiler gives other registers than its split needs is refused where it is launched; what
+    prepares a device for every entry fails for the device and for CUDA's errors only."""
+    text = (CSRC / "capi.cu").read_text()
+    prepare = text.split("int prepare_device(int device, int* sm_count) {")[1].split("\n}\n")[0]
+    refusals = [line for line in prepare.splitlines() if "fail(" in line]
+    assert len(refusals) == 2 and "bad device" in refusals[0] and "built for sm_100a" in refusals[1]
+    launch = text.split("int wamffn_cache_attention(void* stream,")[1].split("\n}\n")[0]
+    assert launch.index("registers != kManyLaunchRegs") < launch.index("launch_pdl(kv_attend_many_kernel")

@@ -136,6 +136,7 @@ struct DeviceInfo {
 };
 std::mutex g_dev_mu;
 DeviceInfo g_dev[64];
+std::atomic<int> g_many_registers{0};  // a thread of kv_attend_many_kernel, as it was compiled
 
 // Checks the device is an sm_100 part and raises the kernels' shared-memory limit once.
 int prepare_device(int device, int* sm_count) {
@@ -170,12 +171,9 @@ int prepare_device(int device, int* sm_count) {
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_few_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     WAMFFN_CUDA(cudaFuncSetAttribute(kv_attend_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
-    // The kernel's warpgroups trade registers: a split that the launch does not bring would wait for good.
     cudaFuncAttributes many_attr{};
     WAMFFN_CUDA(cudaFuncGetAttributes(&many_attr, kv_attend_many_kernel));
-    if (many_attr.numRegs != kManyLaunchRegs)
-      return fail(WAMFFN_ERR_UNSUPPORTED, "kv_attend_many_kernel has %d registers, not %d", many_attr.numRegs,
-                  kManyLaunchRegs);
+    g_many_registers.store(many_attr.numRegs, std::memory_order_relaxed);
     cudaFuncAttributes pass_attr{};
     WAMFFN_CUDA(cudaFuncGetAttributes(&pass_attr, stack_pass_kernel));  // its static barriers count too
     WAMFFN_CUDA(cudaFuncSetAttribute(stack_pass_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -2173,6 +2171,10 @@ int wamffn_cache_attention(void* stream, const wamffn_cache_attention_args* a) {
     return fail(WAMFFN_ERR_INVALID, "too many query rows");
   const dim3 grid(unsigned(x), unsigned(p.c.kv_heads), unsigned(p.c.batch));
   if (plan.many) {
+    // The kernel's warpgroups trade registers: a split that the launch does not bring would wait for good.
+    const int registers = g_many_registers.load(std::memory_order_relaxed);
+    if (registers != kManyLaunchRegs)
+      return fail(WAMFFN_ERR_UNSUPPORTED, "kv_attend_many_kernel has %d registers, not %d", registers, kManyLaunchRegs);
     rc = launch_pdl(kv_attend_many_kernel, grid, kManyThreads, kManySmem, p.split, stream, p);
   } else {
     CUtensorMap kmap, vmap;
