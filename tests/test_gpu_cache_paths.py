@@ -283,3 +283,17 @@ def test_recorded_on_tensors_with_data(cuda_device):
     for a, b in zip(recorded(y), step(caches[1], y)):
         assert torch.equal(a, b)
     assert torch.equal(caches[0].keys.view(torch.uint8), caches[1].keys.view(torch.uint8))
+
+
+@pytest.mark.parametrize("nq,heads,kv_heads,length,key_split", MEETINGS)
+def test_huge_queries_and_keys_that_do_not_meet(cuda_device, nq, heads, kv_heads, length, key_split):
+    """Queries of 2^100 in one dim, keys of 2^40 in the others: every score is zero, whatever the product of the two
+    powers of two that stand for them (past fp32's largest number); the values' mean comes out."""
+    cache, g = make(cuda_device, nq, 1, kv_heads, [length], spread=1)
+    keys = cache.keys.float()
+    keys[..., 5] = torch.where(keys[..., 5].isnan(), keys[..., 5], 0.0)
+    cache.keys.copy_(keys.to(cache.keys.dtype))
+    cache.key_scales.fill_(2.0 ** 33)
+    q = torch.zeros(1, nq, heads * DIM, dtype=torch.bfloat16, device=cuda_device)
+    q.view(1, nq, heads, DIM)[..., 5] = 2.0 ** 100
+    close(cache.attend(q, heads, key_split=key_split), attention(Model(cache), q, heads, False), length)

@@ -29,6 +29,8 @@
 // the rows that do see it get it back.
 #pragma once
 
+#include <cfloat>
+
 #include "kvcache.cuh"
 #include "ptx.cuh"
 
@@ -406,7 +408,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
         fence_proxy_async();  // the place is refilled by a bulk copy
         __syncwarp();
       }
-      const float f[2] = {qf[0] * kf, qf[1] * kf}, evf = float(ev);
+      // Finite, so that a product of zero stays zero: two huge powers of two may stand for vectors that do not meet.
+      const float f[2] = {fminf(qf[0] * kf, FLT_MAX), fminf(qf[1] * kf, FLT_MAX)}, evf = float(ev);
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)

@@ -440,7 +440,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           for (int e = 0; e < 4; ++e)
             t[e] = fmaxf(fmaxf(t[e], __uint_as_float(v[i >> 5][(i & 31) + 2 * e])),
                          __uint_as_float(v[i >> 5][(i & 31) + 2 * e + 1]));
-        const float u = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), f = qf * sc.kf;
+        const float u = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        const float f = fminf(qf * sc.kf, FLT_MAX);  // finite: a product of zero stays zero
         // A block that is not there has ev -inf; nothing seen leaves u at -inf.
         const float top = u == -INFINITY ? -INFINITY : fmaf(u, f, sc.ev);
         // A maximum that grows by at most 2^kLag is left as it is.
