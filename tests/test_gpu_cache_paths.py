@@ -297,3 +297,19 @@ def test_huge_queries_and_keys_that_do_not_meet(cuda_device, nq, heads, kv_heads
     q = torch.zeros(1, nq, heads * DIM, dtype=torch.bfloat16, device=cuda_device)
     q.view(1, nq, heads, DIM)[..., 5] = 2.0 ** 100
     close(cache.attend(q, heads, key_split=key_split), attention(Model(cache), q, heads, False), length)
+
+
+@pytest.mark.parametrize("nq", [1, 12, 40, 300])
+def test_queries_of_nan_over_blocks_that_are_left_out(cuda_device, nq):
+    """A row whose every block lies outside the pool sees nothing: zeros, whatever the query holds; in a sequence with
+    one good block it sees that."""
+    cache, g = make(cuda_device, nq, 3, 1, [130, 130, 64], spread=1)
+    cache.block_table[0] = torch.tensor([-1, 999, 1 << 30], dtype=torch.int32)
+    cache.block_table[1, 1:] = -7
+    q = rows(g, 3, nq, 2 * DIM)
+    q[:, 0, :DIM] = float("nan")
+    q[:, 0, DIM] = float("inf")
+    for split in (0, 1, 2):
+        out = cache.attend(q, 2, key_split=split)
+        assert cache.status() == 2
+        assert not out[0].any() and out[1:, 0].isnan().all() and out[1:, 1:].isfinite().all()

@@ -426,8 +426,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         const int key0 = (first + j) * kManyStep;
         tmem_wait_ld(v[0]);
         tmem_wait_ld(v[1]);
-        if (key0 + kManyStep > least) {  // some row of the CTA sees less than the whole step
-          const int limit = seen - key0;
+        // Some row of the CTA sees less than the whole step, or no row sees a block that is not there (its zeros
+        // would be NaN to a query of NaN).
+        if (key0 + kManyStep > least || sc.there == 0.f) {
+          const int limit = sc.there == 0.f ? 0 : seen - key0;
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (i >= limit) v[i >> 5][i & 31] = 0xff800000u;  // -inf
