@@ -61,3 +61,19 @@ def test_calls_are_recorded_by_a_tracer():
     names = [str(n.target).split(".")[1] for n in graph.nodes if str(n.target).startswith("wam_ffn.")]
     assert names == ["qk_norm_rope", "q_norm_rope", "cache_append", "cache_append", "cache_attention",
                      "cache_attention", "cache_read", "cache_read"]
+
+
+def test_gradients_are_refused_in_traced_calls_too():
+    """A traced append would take the rows and lose their gradient."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, cache, *_ = fakes()
+        k = x[..., :256].contiguous()
+        wants = k.clone().requires_grad_()
+        for call in (lambda: cache.append(wants, k), lambda: cache.append(k, wants), lambda: cache.attend(wants, 2)):
+            with pytest.raises(RuntimeError, match="backward"):
+                call()
+        with torch.no_grad():
+            cache.append(wants, wants)
+            assert cache.attend(wants, 2).shape == wants.shape

@@ -30,6 +30,13 @@ HEAD_DIM = 128
 FORMAT = torch.float8_e4m3fn
 
 
+def _no_gradients(*tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError("the 8-bit cache has no backward pass: run it with gradients disabled")
+
+
 def _rows(t: torch.Tensor, name: str, batch: int, width: int,
           device: torch.device) -> tuple[_lib.RowsView, torch.Tensor]:
     """View of a [batch, rows, width] bf16 operand, and the tensor it views (a
@@ -39,8 +46,6 @@ def _rows(t: torch.Tensor, name: str, batch: int, width: int,
     count, rows, held = t.shape
     if count != batch or held != width:
         raise ValueError(f"{name} {tuple(t.shape)}: expected [{batch}, rows, {width}]")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("the 8-bit cache has no backward pass: run it with gradients disabled")
     sb, sr, se = t.stride()
     if se != 1 or (count > 1 and sb % 8) or (rows > 1 and (sr % 8 or sr < width)) or t.data_ptr() % 16:
         t = t.contiguous()
@@ -216,6 +221,7 @@ class KVCache8:
         rounded to the new one.  A sequence whose rows do not fit (past capacity, ``at``
         beyond its length, a block id outside the pool) keeps what it had, and
         ``status`` reports it."""
+        _no_gradients(k, v)
         if _lib.traced(k):
             return _append_op(k, v, counts, at, *self._tensors())
         self._append(k, v, counts, at)
@@ -261,6 +267,7 @@ class KVCache8:
         row that sees nothing is zeros.  NaN comes out where a row sees it: of a
         query or key in the whole of its heads, of a value in its dim.  key_split:
         CTAs of a cluster sharing a query tile's keys (0 = chosen; 1, 2, 4, 8)."""
+        _no_gradients(q)
         if _lib.traced(q):
             return _attend_op(q, heads, causal, key_split, *self._tensors())
         return self._attend(q, heads, causal, key_split)
