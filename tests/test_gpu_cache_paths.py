@@ -313,3 +313,29 @@ def test_queries_of_nan_over_blocks_that_are_left_out(cuda_device, nq):
         out = cache.attend(q, 2, key_split=split)
         assert cache.status() == 2
         assert not out[0].any() and out[1:, 0].isnan().all() and out[1:, 1:].isfinite().all()
+
+
+def test_a_prefix_read_back_for_the_current_frame(cuda_device):
+    """Rows stored in 8 bits, read back and handed to the bf16 current-frame attention beside rows of the frame; its
+    probabilities are bf16: 2^-9 of A each on top of the result's rounding."""
+    from waminfer_b200.attention import current_frame_attention
+    from waminfer_b200.cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    heads, prefix, frame, action = 3, 150, 40, 16
+    cache = KVCache8(1, 200, heads, cuda_device)
+    cache.append(rows(g, 1, prefix, heads * DIM), rows(g, 1, prefix, heads * DIM))
+    qv, kv, vv = (rows(g, 1, frame, heads * DIM) for _ in range(3))
+    qa, ka, va = (rows(g, 1, action, heads * DIM) for _ in range(3))
+    ck, cv = cache.read(prefix)
+    got = torch.cat(current_frame_attention(qv, qa, ck, kv, ka, cv, vv, va, heads), 1).cpu().double()
+    model = Model(cache)
+    k = torch.cat((torch.stack([model.rows(0, 0, h) for h in range(heads)], 1),
+                   torch.cat((kv, ka), 1)[0].cpu().double().view(-1, heads, DIM)))
+    v = torch.cat((torch.stack([model.rows(1, 0, h) for h in range(heads)], 1),
+                   torch.cat((vv, va), 1)[0].cpu().double().view(-1, heads, DIM)))
+    q = torch.cat((qv, qa), 1)[0].cpu().double().view(-1, heads, DIM)
+    p = torch.softmax(torch.einsum("ihd,jhd->hij", q, k) / DIM ** 0.5, -1)
+    out = torch.einsum("hij,jhd->ihd", p, v).reshape(got.shape)
+    absolute = torch.einsum("hij,jhd->ihd", p, v.abs()).reshape(got.shape)
+    assert ((got - out).abs() <= 2.0 ** -8 * out.abs() + (2.0 ** -8 + 2.0 ** -12) * absolute).all()
