@@ -421,7 +421,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
           x[j][e] = v;
           top[slot(e)] = fmaxf(top[slot(e)], v);
         }
-      // A maximum that grows by at most 2^kLag is left as it is: P stays below f16's range.
+      // The first maximum needs no correction; one that grows by at most 2^kLag is left as it is: P stays below f16's
+      // range.
       bool apart[2];
       float base[2], sum[2] = {0.f, 0.f}, back[2] = {exp2_int(-ev), exp2_int(-ev)};
 #pragma unroll
@@ -429,8 +430,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3)
 #pragma unroll
         for (int w = kNarrow ? 4 : 1; w < (kNarrow ? 32 : 4); w <<= 1)
           top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], w));
-        apart[half] = top[half] > -INFINITY &&
-                      (top[half] > m[half] + kLag || top[half] < m[half] - kDeep || m[half] == -INFINITY);
+        if (m[half] == -INFINITY) m[half] = top[half];
+        apart[half] = top[half] > m[half] + kLag || (top[half] < m[half] - kDeep && top[half] > -INFINITY);
         const float ref = apart[half] ? top[half] : m[half];
         base[half] = kPBias - (ref == -INFINITY ? 0.f : ref);
       }

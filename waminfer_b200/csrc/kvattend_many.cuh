@@ -446,18 +446,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
         const float f = fminf(qf * sc.kf, FLT_MAX);  // finite: a product of zero stays zero
         // A block that is not there has ev -inf; nothing seen leaves u at -inf.
         const float top = u == -INFINITY ? -INFINITY : fmaf(u, f, sc.ev);
-        // A maximum that grows by at most 2^kLag is left as it is.
-        const bool grown = top > m + kLag || (m == -INFINITY && top > m);
-        float corr = 1.f;
-        if (grown) {
-          const float fold = ex2_approx(0.5f * (m - top));
-          corr = fold * fold;
-          m = top;
-          l = folded(l, fold);
-        }
-        const bool deep = top < m - kDeep && top > -INFINITY;
-        const bool rare = __any_sync(0xffffffffu, grown || deep);
-        const float ref = deep ? top : m;
+        // The first maximum needs no correction; one that grows by at most 2^kLag is left as it is.
+        if (m == -INFINITY) m = top;
+        const bool apart = top > m + kLag || (top < m - kDeep && top > -INFINITY);
+        const bool rare = __any_sync(0xffffffffu, apart);
+        const float ref = apart ? top : m;
         const float base = sc.ev - (ref == -INFINITY ? 0.f : ref) + kPBias;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t out[32];
@@ -470,21 +463,28 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
           sum[i & 1] = add2(sum[i & 1], e);
           out[i] = f16x2_pack(e.x, e.y);
         }
-        float back = sc.back;
+        float back = sc.back, corr = 1.f;
         if (rare) {
-          if (deep) {  // the sum alone gets these (kvattend.cuh)
-            const float fold = ex2_approx(0.5f * (top - m - sc.ev));
-            back = fold;
-            sum[0] = make_float2((sum[0].x + sum[1].x) * fold, (sum[0].y + sum[1].y) * fold);
-            sum[1] = make_float2(0.f, 0.f);
+          if (apart) {
+            const bool grown = top > m;
+            const float fold = ex2_approx(0.5f * (grown ? m - top : top - m - sc.ev));
+            if (grown) {
+              corr = fold * fold;
+              l = folded(l, fold);
+              m = top;
+            } else {  // deep: the sum alone gets these (kvattend.cuh)
+              back = fold;
+              sum[0] = make_float2((sum[0].x + sum[1].x) * fold, (sum[0].y + sum[1].y) * fold);
+              sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) out[i] = 0u;
+              for (int i = 0; i < 32; ++i) out[i] = 0u;
+            }
           }
           __syncwarp();
         }
         tmem_st32(ts, out);
         l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), back, l);
-        if (rare && n > 0 && __any_sync(0xffffffffu, grown)) {
+        if (rare && __any_sync(0xffffffffu, corr != 1.f)) {  // not in the first step: m was new
           if (lane == 0)
             ok = wait_spin(smem_addr(&sh.o_step[x]), uint32_t(n - 1) & 1u, abort, c.status, WAMFFN_DEV_TIMEOUT);
           ok = warp_verdict(ok);
