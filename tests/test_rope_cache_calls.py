@@ -77,3 +77,21 @@ def test_gradients_are_refused_in_traced_calls_too():
         with torch.no_grad():
             cache.append(wants, wants)
             assert cache.attend(wants, 2).shape == wants.shape
+
+
+def test_a_cache_takes_attributes_of_the_program():
+    """Only what the calls go by is fixed."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        _, cache, *_ = fakes()
+    cache.step = 0
+    cache.step += 1
+    assert cache.step == 1
+    del cache.step
+    assert not hasattr(cache, "step")
+    for name in ("lengths", "batch", "_view"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, object())
+        with pytest.raises(AttributeError, match=name):
+            delattr(cache, name)

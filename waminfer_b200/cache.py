@@ -28,6 +28,9 @@ from waminfer_b200 import _lib
 BLOCK = 64
 HEAD_DIM = 128
 FORMAT = torch.float8_e4m3fn
+# What a cache's calls go by from when it was made.
+_FIXED = frozenset(("keys", "values", "key_scales", "value_scales", "block_table", "lengths", "batch", "width",
+                    "kv_heads", "device", "_work", "_view", "_needs"))
 
 
 def _no_gradients(*tensors: torch.Tensor) -> None:
@@ -187,13 +190,15 @@ class KVCache8:
             keys, values, key_scales, value_scales, block_table, lengths, self._work)
 
     def __setattr__(self, name, value):
-        if name in self.__dict__ and value is not self.__dict__[name]:  # x += 1 binds the same tensor again
+        if name in _FIXED and name in self.__dict__ and value is not self.__dict__[name]:  # not x += 1, in place
             raise AttributeError(f"{name} of a cache cannot be replaced: write into it, or make another cache "
                                  "(KVCache8.of)")
         object.__setattr__(self, name, value)
 
     def __delattr__(self, name):
-        raise AttributeError(f"{name} of a cache cannot be deleted")
+        if name in _FIXED:
+            raise AttributeError(f"{name} of a cache cannot be deleted")
+        object.__delattr__(self, name)
 
     def _tensors(self):
         return (self.keys, self.values, self.key_scales, self.value_scales, self.block_table, self.lengths, self._work)
