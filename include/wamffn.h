@@ -539,7 +539,7 @@ int wamffn_current_frame_attention(void* stream, const wamffn_current_frame_args
  *   y = x r weight;  pair (a, b) of a head -> (y_a c - y_b s, y_a s + y_b c)
  * c + i s = rope[position, i], i < pairs; (a, b) = (2i, 2i+1) when interleaved,
  * else (i, i + pairs); dims past 2 pairs are not turned.  fp32 throughout,
- * rounded to bf16 once.
+ * rounded to bf16 once (a mean of squares past fp32's range makes zeros).
  * q: [batch, rows, heads * head_dim], k: [batch, rows, kv_heads * head_dim]
  * (data NULL with kv_heads 0: queries only), row and batch strides in elements,
  * multiples of 8.  Weights: head_dim values, or with whole_row the row's width.
@@ -649,7 +649,7 @@ int wamffn_cache_read(void* stream, const wamffn_cache_read_args* args);
 /* out[b, i, h] = softmax over the rows j that query i sees of
  * (q[b, i, h] . k[j] / sqrt(128)) . v[j]: j < lengths[b], or with causal
  * j < lengths[b] - nq + i + 1 (the queries are the cache's last nq rows); a row
- * that sees nothing is zeros.  q: [batch, nq, heads * 128] bf16 (strides
+ * that sees nothing (or whose every score is -inf) is zeros.  q: [batch, nq, heads * 128] bf16 (strides
  * multiples of 8), heads a multiple of the cache's kv_heads: query heads
  * [g * heads / kv_heads, ...) share key head g.  out contiguous.  fp32 scores,
  * maximum, sums, every key counted in the normaliser whatever its values' scale;
@@ -661,7 +661,8 @@ int wamffn_cache_read(void* stream, const wamffn_cache_read_args* args);
  * kernel puts together: workspace (16-byte aligned, the call's own while it runs)
  * holds them.  Without one, or with fewer bytes than
  * wamffn_cache_attention_workspace names for the same arguments, the call does
- * with fewer parts. */
+ * with fewer parts.  The lengths are on the device, so the work is shared out for
+ * the table's width: a table much wider than the rows held costs time. */
 typedef struct wamffn_cache_attention_args {
   wamffn_cache_view cache;
   wamffn_rows_view q;

@@ -194,10 +194,11 @@ __device__ __forceinline__ uint4 clean_chunk(uint4 u, int key, int length, bool 
 // 16 dims of four rows of V), so nothing is written back to shared memory.
 // Up to 8 rows stand as the products' columns (S^T = K Q^T, O^T = V^T P^T: half the
 // instructions of rows as rows, 32 instead of 64 accumulators), up to 16 as their rows.
-// On a B200, 16 x 1 token of 32 heads over up to 16381 rows of 8 key heads: 66 us, 82 %
+// On a B200, 16 x 1 token of 32 heads over up to 16381 rows of 8 key heads: 67 us, 80 %
 // of the measured copy bandwidth (80 us with rows as rows; 94 us with two CTAs an
-// SM; 89 % where all sequences are equally long); one token over 577 rows of 24
-// heads 6 us, latency: length and block ids, then the rows, then two reductions.
+// SM; 88 % where all sequences are equally long, two thirds with 12 packed rows, as rows); one
+// token over 577 rows of 24 heads 6 us, latency: length and block ids, then the rows, then
+// two reductions.
 // Four warps with rings and units of their own, three CTAs an SM (a unit is one
 // long chain of dependent steps, and warps hide each other's);
 // a cluster of `split` CTAs shares the keys of a part, and the partial results meet

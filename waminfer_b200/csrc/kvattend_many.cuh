@@ -2,9 +2,11 @@
 // formulas and the numbers): tcgen05, 256 packed rows (query token x head of
 // the group) a CTA as two tiles of 128, a step of 64 keys (one block).
 //
-// Bound: the tensor cores and the exponentials, about even (512 flops and one
-// exp2 a (row, key); 4096 f16 multiply-adds and 16 exp2 a clock and SM make 128
-// rows x 64 keys 512 clocks of either), with shared memory close behind.  So
+// Bound: shared memory, then the tensor cores and the exponentials (512 flops and one
+// exp2 a (row, key); 4096 f16 multiply-adds and 16 exp2 a clock and SM make two tiles
+// of 128 rows x 64 keys 1024 clocks of either).  A step of two tiles moves 192 KB through
+// shared memory: the products 128 (S: Q 64 and K 32; P V: V 32), the block's copy 16, its
+// conversion 16 in and 32 out; at 128 bytes a clock 1536 clocks.  So
 //   - a converted block serves both tiles; a CTA with at most 128 rows has them in both,
 //     the even steps in one and the odd steps in the other;
 //   - each tile has two S buffers: S of step j + 1 is there before P of step j is,
@@ -13,12 +15,14 @@
 //     conversion.  (Loads to registers instead are slower the further ahead they are:
 //     the fence between a conversion's stores and the products waits for them.)
 //
-// On a B200, 512 queries of 37 heads over 16384 rows (every SM busy) run at 875 TFLOP/s,
-// 53 % of the measured bf16 GEMM burst, the tensor pipe 45 % and the exponentials'
-// 46 % of the cycles; 392 queries of 24 heads over 32768 rows take 215 us.  A step of
-// both tiles takes 1.2 us: the chain of a tile's products, row maximum and exponentials
-// (P of step j must be read before S of step j + 2 takes its columns; TMEM has no
-// room for a third buffer).
+// On a B200, 512 queries of 37 heads over 16384 rows (every SM busy) take 161 us, 989
+// TFLOP/s, 60 % of the measured bf16 GEMM burst; 392 queries of 24 heads over 32768 rows
+// 215 us (232 once the card is at its power limit).  Of the 2310 clocks of a step the
+// counters show shared memory's data pipe busy for 1620 (70 %: 1024 wavefronts of the
+// products, 600 of the warps) beside the bulk copies, the tensor pipe for 44 %, the
+// exponentials' for 45 %.  What stretches a step beyond them is the chain of a tile's
+// products, row maximum and exponentials (P of step j must be read before S of step j + 2
+// takes its columns; TMEM has no room for a third buffer).
 //
 //   warps 8-11, 12-15  softmax of tile 0 and 1, a query row a thread: Q to f16 in shared
 //                   memory once; per step the row maximum, P = 2^(x - m) in f16 over
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
   const int shares = split * p.parts, share = int(blockIdx.x) % shares;  // of the keys: rank of the cluster in its part
   const int rank = share % split, part = share / split;
   // In the order of launch: with a causal mask the last row tile, which has the most keys, of every head, then the one
-  // before, so that the short ones even out the end (16384 rows over 4096: 167 us; 194 us head by head); without one
+  // before, so that the short ones even out the end (16384 rows over 4096: 174 us; head by head 16 % more); without one
   // head by head, whose CTAs then read the same blocks (392 queries over 32768 rows: 215 us; 216 us tile by tile).
   const int tiles = int(gridDim.x) / shares, unit = int(blockIdx.y) * tiles + int(blockIdx.x) / shares;
   const int b = blockIdx.z, kh = p.causal ? unit % int(gridDim.y) : int(blockIdx.y);

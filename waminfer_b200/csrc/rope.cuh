@@ -12,13 +12,16 @@
 // in fp32, rounded to bf16 once (the reference rounds after the norm, after the
 // weight and after the rotation; one rounding is nearer to the formula).
 //
-// Bound: HBM, 4 bytes an element: 2 x 8191 tokens of 32 + 8 heads take 53.7 us on a
-// B200, 98 % of its measured copy bandwidth, norm of each head (up to 8 heads a
+// Bound: HBM, 4 bytes an element: 2 x 8191 tokens of 32 + 8 heads take 54.0 us on a
+// B200, 97 % of its measured copy bandwidth, norm of each head (up to 8 heads a
 // group of lanes; 59 us with 4, 74 us with 2: fewer loads in flight, the table's
-// entries and addresses made for fewer heads).  One token takes 3 us: latency.  A lane holds 8 dims of a head in registers
-// (16 bytes in, 16 out) as two runs of 4, laid so that both members of every
-// pair are in the lane: the rotation needs no exchange.  A lane keeps its dims
-// for all the heads it visits, so its 4 table entries are read once.
+// entries and addresses made for fewer heads); with the norm over the row 90 us, 59 %
+// (a CTA a token, whose loads wait for the one block-wide sum).  One token takes 3 us:
+// latency.  A lane holds 8 dims of a head in registers (16 bytes in, 16 out) as two
+// runs of 4, laid so that both members of every pair are in the lane: the rotation
+// needs no exchange.  A lane keeps its dims for all the heads it visits, so its 4 table
+// entries are read once.  A sum of squares past fp32's range (values beyond some 1e18)
+// is infinite, and the row or head zeros.
 #pragma once
 
 #include "ptx.cuh"
@@ -115,7 +118,7 @@ __device__ __forceinline__ void rope_store(__nv_bfloat16* head, const RopeDims& 
   for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
   // Pairs inside the lane: (0,1)(2,3)(4,5)(6,7) interleaved, (0,4)(1,5)(2,6)(3,7) in halves.
   // An unturned lane's dims are no pairs: an infinity or NaN of one must not reach the other (0 x inf).
-  // (Selects cost 0.3 us of 56 called in the prompt case above, a branch around the products 1.5.)
+  // (Selects cost 0.3 us in the case above, a branch around the products 1.5.)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int a = kInterleaved ? 2 * i : i, b = kInterleaved ? 2 * i + 1 : i + 4;
